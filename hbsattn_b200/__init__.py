@@ -14,9 +14,12 @@ from .hbsa_interface import (HBSAttention, HBSAttention_csr, attention_backward,
                              block_decisions, block_decisions_csr, build_schedule, last_status, set_kernel_family)
 from .utils import calculate_blocks  # noqa: E402
 from .host_staged import HostStagedAttention  # noqa: E402
+from .paged_cache import (append_to_cache, attention_key_weights, attention_key_weights_csr, compact_cache, paged_attention,  # noqa: E402
+                          select_keys)
 
 __all__ = ["HBSAttention", "calculate_blocks", "block_decisions", "last_status", "set_kernel_family",
-           "HBSAttention_with_lse", "HBSAttention_csr", "block_decisions_csr", "attention_backward", "HostStagedAttention", "MaskSchedule", "build_schedule", "attention_with_schedule", "install_as_hbsattn"]
+           "HBSAttention_with_lse", "HBSAttention_csr", "block_decisions_csr", "attention_backward", "HostStagedAttention", "MaskSchedule", "build_schedule", "attention_with_schedule", "install_as_hbsattn",
+           "append_to_cache", "paged_attention", "attention_key_weights", "attention_key_weights_csr", "select_keys", "compact_cache"]
 
 
 def install_as_hbsattn(reference_package_dir=None) -> None:

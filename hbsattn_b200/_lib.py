@@ -15,7 +15,7 @@ LIB_PATH = os.environ.get("HBSATTN_B200_LIBRARY") or os.path.join(PKG_DIR, "libh
 
 HBSA_DTYPE_BF16, HBSA_DTYPE_F16, HBSA_DTYPE_F32 = 0, 1, 2
 HBSA_IMPL_AUTO, HBSA_IMPL_GENERIC, HBSA_IMPL_SM100 = 0, 1, 2
-HBSA_STATUS_OK, HBSA_STATUS_BLOCK_COUNT_MISMATCH, HBSA_STATUS_WAIT_LIMIT = 0, 1, 2
+HBSA_STATUS_OK, HBSA_STATUS_BLOCK_COUNT_MISMATCH, HBSA_STATUS_WAIT_LIMIT, HBSA_STATUS_CACHE_BOUNDS = 0, 1, 2, 3
 STATUS_WORDS = 16
 
 EXPORTED_SYMBOLS = (
@@ -38,6 +38,13 @@ EXPORTED_SYMBOLS = (
     "hbsa_debug_set_wait_budget",
     "hbsa_debug_trace_bytes",
     "hbsa_debug_set_trace",
+    "hbsa_append_to_cache",
+    "hbsa_paged_attention",
+    "hbsa_paged_attention_workspace_bytes",
+    "hbsa_key_weights",
+    "hbsa_key_weights_workspace_bytes",
+    "hbsa_select_keys",
+    "hbsa_compact_cache",
 )
 STATIC_SCRATCH_BYTES = 4 << 20
 
@@ -99,6 +106,35 @@ class BackwardArgs(ctypes.Structure):
     ]
 
 
+def _mirror(name, *fields):
+    return type(name, (ctypes.Structure,), {"_fields_": [("struct_bytes", ctypes.c_size_t), *fields], "__doc__": f"Mirror of ``struct {name}``."})
+
+
+_p, _i, _l = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64
+
+
+class Cache(ctypes.Structure):
+    """Mirror of ``struct hbsa_cache``."""
+
+    _fields_ = [("k", _p), ("v", _p), ("k_stride", _l * 4), ("v_stride", _l * 4), ("block_table", _p), ("table_stride", _l), ("lens", _p),
+                ("num_pages", _i), ("page_size", _i), ("max_pages", _i), ("batch", _i), ("nhead_k", _i), ("headdim", _i), ("dtype", _i),
+                ("reserved", _i)]
+
+
+AppendArgs = _mirror("hbsa_append_args", ("cache", Cache), ("k", _p), ("v", _p), ("k_stride", _l * 3), ("v_stride", _l * 3),
+                     ("cu_seqlens", _p), ("new_lens", _p), ("status", _p), ("total", _i), ("reserved", _i))
+PagedAttentionArgs = _mirror("hbsa_paged_attention_args", ("cache", Cache), ("q", _p), ("o", _p), ("q_stride", _l * 3), ("o_stride", _l * 3),
+                             ("block_mask", _p), ("mask_stride", _l * 3), ("lse", _p), ("key_weights", _p), ("weights_stride", _l * 2),
+                             ("nhead_q", _i), ("num_k_block", _i), ("k_block_size", _i), ("use_default_scale", _i),
+                             ("softmax_scale", ctypes.c_float), ("impl", _i), ("workspace", _p), ("workspace_bytes", ctypes.c_size_t))
+KeyWeightsArgs = _mirror("hbsa_key_weights_args", ("fwd", ForwardArgs), ("weights", _p), ("partial_workspace", _p),
+                         ("partial_workspace_bytes", ctypes.c_size_t))
+SelectKeysArgs = _mirror("hbsa_select_keys_args", ("key_weights", _p), ("weights_stride", _l * 2), ("lens", _p), ("kept", _p),
+                         ("kept_lens", _p), ("batch", _i), ("nhead_k", _i), ("max_len", _i), ("budget", _i), ("n_sink", _i),
+                         ("n_recent", _i))
+CompactArgs = _mirror("hbsa_compact_args", ("cache", Cache), ("kept", _p), ("kept_lens", _p), ("key_weights", _p),
+                      ("weights_stride", _l * 2), ("budget", _i), ("reserved", _i))
+
 _lock = threading.Lock()
 _lib = None
 
@@ -153,6 +189,13 @@ def load() -> ctypes.CDLL:
         lib.hbsa_debug_set_trace.argtypes = [vp]
         lib.hbsa_debug_set_wait_budget.restype = None
         lib.hbsa_debug_set_wait_budget.argtypes = [ctypes.c_longlong, i32]
+        for name, args in (("hbsa_append_to_cache", AppendArgs), ("hbsa_paged_attention", PagedAttentionArgs), ("hbsa_key_weights", KeyWeightsArgs),
+                           ("hbsa_select_keys", SelectKeysArgs), ("hbsa_compact_cache", CompactArgs)):
+            getattr(lib, name).restype = i32
+            getattr(lib, name).argtypes = [ctypes.POINTER(args), vp]
+        for name, args in (("hbsa_paged_attention_workspace_bytes", PagedAttentionArgs), ("hbsa_key_weights_workspace_bytes", KeyWeightsArgs)):
+            getattr(lib, name).restype = ctypes.c_size_t
+            getattr(lib, name).argtypes = [ctypes.POINTER(args)]
         if lib.hbsa_version() != 4:
             raise ImportError("libhbsattn_b200.so was built from a different ABI version")
         _lib = lib

@@ -20,8 +20,12 @@ int fail_cuda(cudaError_t e, const char* where) {
   return (int)e;
 }
 
+}  // namespace
+
+namespace hbsa {
+
 // Validates everything that does not need the device and fills the kernel-side description.
-int make_problem(const hbsa_forward_args* a, bool need_tensors, hbsa::Problem* p) {
+int make_problem(const hbsa_forward_args* a, bool need_tensors, Problem* p) {
   if (!a) return fail(HBSA_ERR_NULL, "args is NULL");
   if (a->struct_bytes != sizeof(hbsa_forward_args)) return fail(HBSA_ERR_STRUCT, "hbsa_forward_args.struct_bytes does not match this library");
   if (!a->cu_q_seqlens || !a->cu_k_seqlens || !a->workspace)
@@ -41,7 +45,7 @@ int make_problem(const hbsa_forward_args* a, bool need_tensors, hbsa::Problem* p
     return fail(HBSA_ERR_DTYPE, "unknown dtype");
   if (a->impl != HBSA_IMPL_AUTO && a->impl != HBSA_IMPL_GENERIC && a->impl != HBSA_IMPL_SM100)
     return fail(HBSA_ERR_DTYPE, "unknown impl");
-  if (a->workspace_bytes < hbsa::workspace_bytes(a->nhead_k, a->num_q_block, a->num_k_block, a->batch))
+  if (a->workspace_bytes < workspace_bytes(a->nhead_k, a->num_q_block, a->num_k_block, a->batch))
     return fail(HBSA_ERR_WORKSPACE, "workspace is smaller than hbsa_workspace_bytes()");
   if (((uintptr_t)a->workspace) % 256 != 0) return fail(HBSA_ERR_WORKSPACE, "workspace must be 256-byte aligned");
   p->cu_q = a->cu_q_seqlens;
@@ -63,13 +67,13 @@ int make_problem(const hbsa_forward_args* a, bool need_tensors, hbsa::Problem* p
   p->kbs = a->k_block_size;
   p->causal = a->causal ? 1 : 0;
   p->scale = a->use_default_scale ? 1.0f / sqrtf((float)a->headdim) : a->softmax_scale;
-  p->kv_tile = hbsa::kFwdTileRows;
-  p->kv_unit = hbsa::kFwdUnitRows;
+  p->kv_tile = kFwdTileRows;
+  p->kv_unit = kFwdUnitRows;
   return 0;
 }
 
-int select_impl(const hbsa_forward_args* a, const hbsa::Problem& p) {
-  const char* why = hbsa::sm100_ineligible_reason(*a, p.scale);
+int select_impl(const hbsa_forward_args* a, const Problem& p) {
+  const char* why = sm100_ineligible_reason(*a, p.scale);
   if (a->impl == HBSA_IMPL_GENERIC) return HBSA_IMPL_GENERIC;
   if (a->impl == HBSA_IMPL_SM100) {
     if (why) {
@@ -80,6 +84,13 @@ int select_impl(const hbsa_forward_args* a, const hbsa::Problem& p) {
   }
   return why ? HBSA_IMPL_GENERIC : HBSA_IMPL_SM100;
 }
+
+}  // namespace hbsa
+
+namespace {
+
+using hbsa::make_problem;
+using hbsa::select_impl;
 
 // Mapped host memory a kernel reports to, so that a call that has to wait for a few words neither copies them nor waits for the
 // stream's own completion machinery.  One block per host thread, reused by its calls one after the other and freed with the

@@ -164,6 +164,10 @@ struct SmemOptIn {
 // printf-style setter of the text hbsa_last_error() returns on the calling thread.
 void set_last_error(const char* fmt, ...);
 
+// Checks of a forward call and its kernel-side description (0, or HBSA_ERR_* with the error text set), and the kernel family it runs on.
+int make_problem(const hbsa_forward_args* a, bool need_tensors, Problem* p);
+int select_impl(const hbsa_forward_args* a, const Problem& p);
+
 // Launchers (each enqueues on `stream` and returns the cudaError_t of the launch).
 cudaError_t launch_calculate_blocks(const int32_t* cu_seqlen, int batch, int block_size, int capacity,
                                     int32_t* cu_block, int32_t* block_to_batch, int32_t* cu_num_block,

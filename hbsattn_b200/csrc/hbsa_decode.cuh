@@ -1,0 +1,208 @@
+// What the kernels of the paged decode attention share: the description of a call, the split of its work, and the layout of
+// the partial results.
+//
+// One row = one (sequence, kv-head, chunk of at most 32 q-heads of its group).  A row's keys come in tiles of 64; without a
+// block mask tile i holds positions 64 i .. 64 i + 63, with one the tile is strung together from pieces of `unit` positions of the
+// active blocks.  The tiles of all rows stand in one line (sequence, kv-head, chunk, tile), and CTA c of G takes the tiles
+// [c T / G, (c + 1) T / G): every CTA reads the same number of keys, whatever the lengths are, and at most its first and its
+// last row are shared with neighbours.  Those leave (maximum, sum, unnormalised output) in two slots of the CTA's own, which the
+// join kernel puts together in the order of the CTAs, so that results do not depend on timing.
+#pragma once
+#include "hbsa_common.cuh"
+
+namespace hbsa {
+
+constexpr int kDecodeTile = 64;          // keys of a tile
+constexpr int kDecodeHeads = 32;         // q-heads of a row, at most
+constexpr float kDecodeLog2e = 1.4426950408889634f;
+constexpr float kDecodeLn2 = 0.6931471805599453f;
+
+// Carved out of the caller's workspace; all pointers device pointers, each part 256-byte aligned.
+struct DecodeSpace {
+  int32_t* status;           // [kStatusWords], written by the join kernel
+  int32_t* cta_status;       // [G][2] what CTA c has to report: HBSA_STATUS_*, sequence
+  int4* cta_start;           // [G] {row's sequence, kv-head * n_chunk + chunk, tiles of the row before the CTA's first, tiles of the row}
+  long long* entry_start;    // [entries + 1] first tile of every entry (a sequence, or a (sequence, kv-head) where there is a mask)
+  int32_t* pieces;           // [batch * nhead_k] pieces of the active blocks (mask)
+  int32_t* list;             // [batch * nhead_k][num_k_block] the active blocks, ascending (mask)
+  float* lse;                // [batch, nhead_q] (weights, where the caller wants no lse)
+  float* part_ml;            // [2 G][kDecodeHeads][2] maximum (log2 domain) and sum
+  float* part_o;             // [2 G][kDecodeHeads][d_pad]
+  float* scores;             // [batch, nhead_q, capacity] scaled scores in the log2 domain (weights)
+};
+
+struct DecodeParams {
+  DecodeSpace sp;
+  const void *k, *v, *q;
+  void* o;
+  long long k_s[4], v_s[4], q_s[3], o_s[3];
+  const int32_t* table;
+  long long table_stride;
+  const int32_t* lens;
+  const uint8_t* mask;
+  long long mask_s[3];
+  float* lse;                // the caller's, or the workspace's, or NULL
+  float* weights;
+  long long weights_s[2];
+  int num_pages, page, capacity, batch, nhead_q, nhead_k, group, headdim, d_pad;
+  int n_chunk, chunk_heads;  // chunks of a group, q-heads of every chunk but perhaps the last
+  int kbs, num_k_block;
+  int unit, pieces_per_block;
+  int entries;
+  float scale_log2;
+  long long wait_budget;
+  int debug_stall;
+  int grid;                  // G
+};
+
+// First tile of CTA c, and the CTA that owns tile t (the last c whose first tile is not behind t; it is never an empty one).
+__device__ __forceinline__ long long decode_first(long long c, long long total, int grid) { return c * total / grid; }
+__device__ __forceinline__ int decode_owner(long long t, long long total, int grid) { return (int)(((t + 1) * grid - 1) / total); }
+
+__device__ __forceinline__ int decode_len(const DecodeParams& P, int b) { return max(0, min(P.lens[b], P.capacity)); }
+// Tiles of one row of entry e.
+__device__ __forceinline__ int decode_row_tiles(const DecodeParams& P, int e) {
+  if (P.mask == nullptr) return (decode_len(P, e) + kDecodeTile - 1) / kDecodeTile;
+  return (int)(((long long)P.sp.pieces[e] * P.unit + kDecodeTile - 1) / kDecodeTile);
+}
+__device__ __forceinline__ int decode_entry_rows(const DecodeParams& P) { return P.mask == nullptr ? P.nhead_k * P.n_chunk : P.n_chunk; }
+
+// One row, and the tiles of it that a CTA works on.
+struct DecodeRow {
+  int b, hk, chunk;          // b < 0: no more work
+  int tile0, tiles, row_tiles;
+  int slot;                  // partial slot of the CTA (0, 1), or -1: the row is the CTA's alone
+  int len, pieces, entry;
+};
+
+// Finds the place of the tile line at which a CTA starts; all threads of the block call it.  `walk` (shared) receives the entry
+// that holds `first(total)` and the entry's first tile; returns the total.  `table`: the entries' first tiles go there too.
+struct DecodeWalk {
+  long long total, start, end, entry_start;
+  int entry;
+};
+__device__ __forceinline__ void decode_locate(const DecodeParams& P, int cta, int grid, long long* table, DecodeWalk* walk, long long* scratch) {
+  const int tid = threadIdx.x, n_threads = blockDim.x, lane = tid & 31, warp = tid >> 5, n_warps = (n_threads + 31) >> 5;
+  const int rows = decode_entry_rows(P);
+  const int e0 = (int)((long long)P.entries * tid / n_threads), e1 = (int)((long long)P.entries * (tid + 1) / n_threads);
+  long long sum = 0;
+  for (int e = e0; e < e1; ++e) sum += (long long)decode_row_tiles(P, e) * rows;
+  long long incl = sum;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const long long y = __shfl_up_sync(0xffffffffu, incl, d);
+    if (lane >= d) incl += y;
+  }
+  if (lane == 31) scratch[warp] = incl;
+  __syncthreads();
+  long long before = 0, total = 0;
+  for (int w = 0; w < n_warps; ++w) {
+    if (w < warp) before += scratch[w];
+    total += scratch[w];
+  }
+  before += incl - sum;
+  const long long start = decode_first(cta, total, grid), end = decode_first(cta + 1, total, grid);
+  if (tid == 0) {
+    walk->total = total;
+    walk->start = start;
+    walk->end = end;
+    walk->entry = P.entries;
+    walk->entry_start = total;
+    if (table != nullptr) table[P.entries] = total;
+  }
+  __syncthreads();
+  if (table != nullptr || (start < end && start >= before && start < before + sum)) {
+    long long at = before;
+    for (int e = e0; e < e1; ++e) {
+      if (table != nullptr) table[e] = at;
+      const long long n = (long long)decode_row_tiles(P, e) * rows;
+      if (start < end && start >= at && start < at + n) {
+        walk->entry = e;
+        walk->entry_start = at;
+      }
+      at += n;
+    }
+  }
+  __syncthreads();
+}
+
+// The row that holds tile t, and as much of it as lies before `end`; moves `walk` on to the row's entry.
+__device__ __forceinline__ DecodeRow decode_row_at(const DecodeParams& P, DecodeWalk& walk, long long t) {
+  DecodeRow r;
+  const int rows = decode_entry_rows(P);
+  int tiles = decode_row_tiles(P, walk.entry);
+  while (t >= walk.entry_start + (long long)tiles * rows) {      // t < end <= total: there is such an entry
+    walk.entry_start += (long long)tiles * rows;
+    tiles = decode_row_tiles(P, ++walk.entry);
+  }
+  const int in_entry = (int)((t - walk.entry_start) / tiles);
+  const long long row0 = walk.entry_start + (long long)in_entry * tiles;
+  r.entry = walk.entry;
+  r.b = P.mask == nullptr ? walk.entry : walk.entry / P.nhead_k;
+  const int hc = P.mask == nullptr ? in_entry : walk.entry % P.nhead_k * P.n_chunk + in_entry;
+  r.hk = hc / P.n_chunk;
+  r.chunk = hc % P.n_chunk;
+  r.row_tiles = tiles;
+  r.tile0 = (int)(t - row0);
+  r.tiles = (int)(min(walk.end, row0 + tiles) - t);
+  r.len = decode_len(P, r.b);
+  r.pieces = P.mask == nullptr ? 0 : P.sp.pieces[walk.entry];
+  r.slot = r.tiles == tiles ? -1 : t == walk.start ? 0 : 1;
+  return r;
+}
+
+// Position of piece p of a row with a mask, or -1 behind the last.
+__device__ __forceinline__ int decode_piece_position(const DecodeParams& P, const DecodeRow& r, int p) {
+  if (p >= r.pieces) return -1;
+  return P.sp.list[(long long)r.entry * P.num_k_block + p / P.pieces_per_block] * P.kbs + p % P.pieces_per_block * P.unit;
+}
+
+// The output of sequences that see no key: zeros, lse -inf.  All threads of CTA `cta` of `grid`.
+template <typename T>
+__device__ __forceinline__ void decode_fill_empty(const DecodeParams& P, int cta, int grid) {
+  const int heads = P.mask == nullptr ? P.nhead_q : P.group;
+  for (int e = cta; e < P.entries; e += grid) {
+    if (decode_row_tiles(P, e) != 0) continue;
+    const int b = P.mask == nullptr ? e : e / P.nhead_k, h0 = P.mask == nullptr ? 0 : e % P.nhead_k * P.group;
+    for (int i = threadIdx.x; i < heads * P.headdim; i += blockDim.x)
+      static_cast<T*>(P.o)[b * P.o_s[0] + (h0 + i / P.headdim) * P.o_s[1] + i % P.headdim * P.o_s[2]] = T(0.f);
+    if (P.lse != nullptr)
+      for (int i = threadIdx.x; i < heads; i += blockDim.x) P.lse[(long long)b * P.nhead_q + h0 + i] = -INFINITY;
+  }
+}
+
+// What every CTA of the main kernel writes down for the join: its first row.
+__device__ __forceinline__ void decode_note_start(const DecodeParams& P, const DecodeRow& r) {
+  P.sp.cta_start[blockIdx.x] = make_int4(r.b, r.hk * P.n_chunk + r.chunk, r.tile0, r.row_tiles);
+}
+
+__device__ __forceinline__ void decode_note_status(const DecodeParams& P, int status, int sequence) {
+  P.sp.cta_status[2 * blockIdx.x] = status;
+  P.sp.cta_status[2 * blockIdx.x + 1] = sequence;
+}
+
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+const char* decode_sm100_ineligible_reason(const hbsa_paged_attention_args& a, float scale);
+// The main kernel: every row that one CTA has alone is written, the others leave their parts.
+cudaError_t launch_decode_generic(const DecodeParams& P, int dtype, bool dependent, cudaStream_t stream);
+int launch_decode_sm100(const DecodeParams& P, const hbsa_paged_attention_args& a, bool dependent, cudaStream_t stream, const char** err_text);
+
+// Launch with programmatic stream serialization where `dependent`.
+template <typename... K, typename... A>
+cudaError_t launch_kernel(void (*kernel)(K...), unsigned grid, unsigned block, size_t smem, bool dependent, cudaStream_t stream, const A&... args) {
+  cudaLaunchAttribute attr[1] = {};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = dependent ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+}  // namespace hbsa

@@ -1,0 +1,37 @@
+// What the two kernels of the key weights share (hbsa_key_weights.cu, hbsa_key_weights_sm100.cu).
+#pragma once
+#include "hbsa_common.cuh"
+
+namespace hbsa {
+
+struct KeyWeightsSpace {
+  unsigned long long* cursor;  // [32] word 0: next item, word 1: CTAs that have left
+  float* neg_lse;              // [total_q, nhead_q] -lse log2 e; -inf: the row adds nothing
+};
+
+struct KeyWeightsParams {
+  Problem p;
+  Workspace ws;
+  KeyWeightsSpace sp;
+  float* out;                  // [total_k, nhead_k]
+  int total_q, total_k;
+  float scale_log2;
+  // tensor-core kernel
+  int gp, gp_shift, n_head_sub, tt, nt;      // q-heads of a tile, tiles of heads per group, tokens and rows of a tile
+  int m_rows, n_msub;                        // keys of a stationary tile, tiles per k-block
+  long long total_items;
+  long long wait_budget;
+  int debug_stall;
+};
+
+// Keys outside every sample get zeros, and with a block count mismatch all keys do.  All threads of the grid.
+__device__ __forceinline__ void key_weights_outside(const KeyWeightsParams& P, bool all) {
+  const int lo = all ? 0 : max(0, min(P.p.cu_k[0], P.total_k)), hi = all ? 0 : max(lo, min(P.p.cu_k[P.p.batch], P.total_k));
+  const long long n_cta = (long long)gridDim.x * gridDim.y, cta = (long long)blockIdx.y * gridDim.x + blockIdx.x;
+  const long long first = (long long)lo * P.p.nhead_k, last = (long long)hi * P.p.nhead_k, n = (long long)P.total_k * P.p.nhead_k;
+  for (long long i = cta * blockDim.x + threadIdx.x; i < first + (n - last); i += n_cta * blockDim.x) P.out[i < first ? i : i - first + last] = 0.f;
+}
+
+int launch_key_weights_sm100(KeyWeightsParams& P, const hbsa_forward_args& a, cudaStream_t stream, const char** err_text);
+
+}  // namespace hbsa

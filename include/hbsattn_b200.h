@@ -49,7 +49,9 @@ enum {
   HBSA_STATUS_OK = 0,
   HBSA_STATUS_BLOCK_COUNT_MISMATCH = 1, /* num_q_block/num_k_block differ from what cu_seqlens imply;
                                            no attention is computed and `o` is filled with zeros  */
-  HBSA_STATUS_WAIT_LIMIT = 2            /* a bounded wait inside the attention kernel ran out       */
+  HBSA_STATUS_WAIT_LIMIT = 2,           /* a bounded wait inside the attention kernel ran out       */
+  HBSA_STATUS_CACHE_BOUNDS = 3          /* a paged cache: a length is outside [0, max_pages * page_size] or a page index outside
+                                           [0, num_pages); what lies there is left out. Word 1: the first such sequence   */
 };
 
 /* Library / ABI version (HBSA_ABI_VERSION of the build). */
@@ -266,6 +268,159 @@ int hbsa_forward_static_scratch(const hbsa_forward_args* args, void* stream);
  * status_out[0..15].  Synchronises `stream`; allocates nothing.  Like the entry point it serves, it
  * has no counterpart in the reference. */
 int hbsa_static_scratch_status(int32_t* status_out, void* stream);
+
+/* ------------------------------------------------------------------------------------------------------------------
+ * Paged key-value cache.  The reference has no counterpart: its callers hand over packed keys and values only
+ * (hbsattn/hbsa_interface.py:6-35).
+ *
+ * Keys and values live in pages of page_size positions: element (page, slot, head, dim) at page * stride[0] + slot *
+ * stride[1] + head * stride[2] + dim * stride[3], strides in ELEMENTS.  Position p of sequence b is slot p % page_size of
+ * page block_table[b * table_stride + p / page_size]; lens[b] is the number of positions in use.  Lengths are cut to
+ * [0, max_pages * page_size], and positions whose page index is outside [0, num_pages) take part in nothing; append and
+ * attention report both as HBSA_STATUS_CACHE_BOUNDS.
+ */
+typedef struct hbsa_cache {
+  void* k;
+  void* v;
+  int64_t k_stride[4];
+  int64_t v_stride[4];
+  const int32_t* block_table;     /* int32 [batch, max_pages], unit stride along the second dimension */
+  int64_t table_stride;
+  const int32_t* lens;            /* int32 [batch]                                              */
+  int32_t num_pages;
+  int32_t page_size;
+  int32_t max_pages;              /* max_pages * page_size < 2^31                                 */
+  int32_t batch;
+  int32_t nhead_k;
+  int32_t headdim;                /* <= 256                                                     */
+  int32_t dtype;                  /* HBSA_DTYPE_* of k and v                                    */
+  int32_t reserved;
+} hbsa_cache;
+
+/*
+ * Writes new tokens behind those that a sequence holds already: token i of sequence b, row cu_seqlens[b] + i of k and v
+ * (packed [total, nhead_k, headdim], strides in elements), goes to position cache.lens[b] + i.  Rows of k and v outside
+ * every sequence are not read, positions outside the cache are not written.
+ *   new_lens   int32 [batch]: lens[b] plus the number of its new tokens, cut to the cache's capacity
+ *   status     16 int32 words (device) that hbsa_read_status reads
+ */
+typedef struct hbsa_append_args {
+  size_t struct_bytes;            /* sizeof(hbsa_append_args) of the caller */
+  hbsa_cache cache;
+  const void* k;
+  const void* v;
+  int64_t k_stride[3];
+  int64_t v_stride[3];
+  const int32_t* cu_seqlens;      /* int32 [batch + 1] */
+  int32_t* new_lens;
+  int32_t* status;
+  int32_t total;
+  int32_t reserved;
+} hbsa_append_args;
+
+int hbsa_append_to_cache(const hbsa_append_args* args, void* stream);
+
+/*
+ * Attention of one new token per sequence over its cache: o[b, h] = softmax(scale q[b, h] K_b^T) V_b over the positions
+ * below lens[b], those of active blocks only where a block mask is given.  Sequences that see no key get zeros (lse -inf).
+ *   block_mask    NULL, or bool bytes [batch, nhead_k, num_k_block], strides in BYTES, over blocks of k_block_size positions
+ *                 (a multiple of 16) from the start of every sequence; num_k_block * k_block_size >= max_pages * page_size
+ *   lse           NULL, or float32 [batch, nhead_q] (contiguous): natural-log sum of exponentials of the scaled scores
+ *   key_weights   NULL, or float32 [batch, nhead_k, >= max_pages * page_size], strides in elements (unit along the last):
+ *                 receives, added to what is there, the attention weight of every key summed over the q-heads of its kv-head
+ * The tensor-core kernel takes bf16/fp16, headdim a multiple of 8 from 16 to 256 with unit stride, 16-byte aligned rows, a page
+ * size that is a multiple of 16 and softmax_scale > 0; a CUDA-core kernel takes the rest.  Should a wait inside the former
+ * run out, the status word says HBSA_STATUS_WAIT_LIMIT, o and lse are NaN, and key_weights are left as they were.
+ */
+typedef struct hbsa_paged_attention_args {
+  size_t struct_bytes;            /* sizeof(hbsa_paged_attention_args) of the caller */
+  hbsa_cache cache;
+  const void* q;                  /* [batch, nhead_q, headdim] */
+  void* o;                        /* like q                    */
+  int64_t q_stride[3];
+  int64_t o_stride[3];
+  const uint8_t* block_mask;
+  int64_t mask_stride[3];
+  float* lse;
+  float* key_weights;
+  int64_t weights_stride[2];
+  int32_t nhead_q;
+  int32_t num_k_block;
+  int32_t k_block_size;
+  int32_t use_default_scale;
+  float softmax_scale;
+  int32_t impl;                   /* HBSA_IMPL_* */
+  void* workspace;                /* >= hbsa_paged_attention_workspace_bytes(...) bytes, 256-byte aligned; starts with the status words */
+  size_t workspace_bytes;
+} hbsa_paged_attention_args;
+
+/* Depends on the sizes, the dtype, and on which of block_mask and key_weights are given; asks the current device for its number of SMs. */
+size_t hbsa_paged_attention_workspace_bytes(const hbsa_paged_attention_args* args);
+int hbsa_paged_attention(const hbsa_paged_attention_args* args, void* stream);
+
+/*
+ * The attention weight that the queries of a forward call give to every key, summed over the rows that see it and over the
+ * q-heads of its kv-head: weights[j, hk] = sum exp(scale q.k_j - lse), float32 [total_k, nhead_k] (contiguous).
+ * `fwd` describes the call: q, k, the forward's lse (required), mask, sizes, workspace (the schedule is rebuilt in it); v and
+ * o are not used.  Keys outside every sample get zeros.  Rows whose lse is -inf add nothing.  The tcgen05 kernel runs what
+ * the forward's takes; should a wait inside it run out, the status word says HBSA_STATUS_WAIT_LIMIT and the weights are NaN.
+ * partial_workspace: >= hbsa_key_weights_workspace_bytes(...) bytes, 256-byte aligned.
+ */
+typedef struct hbsa_key_weights_args {
+  size_t struct_bytes;            /* sizeof(hbsa_key_weights_args) of the caller */
+  hbsa_forward_args fwd;
+  float* weights;
+  void* partial_workspace;
+  size_t partial_workspace_bytes;
+} hbsa_key_weights_args;
+
+size_t hbsa_key_weights_workspace_bytes(const hbsa_key_weights_args* args);
+int hbsa_key_weights(const hbsa_key_weights_args* args, void* stream);
+
+/*
+ * Which positions of every sequence and kv-head stay when a cache is cut to `budget`: the first n_sink, the last n_recent,
+ * and those of the largest weight in between (of equal weights the lowest positions; NaN counts as the largest).  Sequences
+ * of at most `budget` positions stay whole.
+ *   key_weights   float32 [batch, nhead_k, max_len], strides in elements, unit along the last; lens are cut to [0, max_len]
+ *   kept          int32 [batch, nhead_k, budget] (contiguous): the positions in ascending order, then -1
+ *   kept_lens     int32 [batch]: min(lens, budget)
+ */
+typedef struct hbsa_select_keys_args {
+  size_t struct_bytes;            /* sizeof(hbsa_select_keys_args) of the caller */
+  const float* key_weights;
+  int64_t weights_stride[2];
+  const int32_t* lens;
+  int32_t* kept;
+  int32_t* kept_lens;
+  int32_t batch;
+  int32_t nhead_k;
+  int32_t max_len;
+  int32_t budget;
+  int32_t n_sink;
+  int32_t n_recent;
+} hbsa_select_keys_args;
+
+int hbsa_select_keys(const hbsa_select_keys_args* args, void* stream);
+
+/*
+ * Moves the kept positions of every sequence and kv-head to its front, in place: position j becomes what position
+ * kept[b, h, j] was, j < kept_lens[b].  The positions have to ascend (as hbsa_select_keys gives them) and pages must not be
+ * shared by sequences, otherwise the contents of the pages are unspecified.  Entries of kept outside [0, lens[b]) move nothing.
+ *   key_weights   NULL, or float32 [batch, nhead_k, >= max_pages * page_size]: moved in the same way, the positions from
+ *                 kept_lens[b] to lens[b] become zero
+ */
+typedef struct hbsa_compact_args {
+  size_t struct_bytes;            /* sizeof(hbsa_compact_args) of the caller */
+  hbsa_cache cache;               /* lens: those before the move */
+  const int32_t* kept;            /* int32 [batch, nhead_k, budget], contiguous */
+  const int32_t* kept_lens;       /* int32 [batch], cut to [0, budget] */
+  float* key_weights;
+  int64_t weights_stride[2];
+  int32_t budget;
+  int32_t reserved;
+} hbsa_compact_args;
+
+int hbsa_compact_cache(const hbsa_compact_args* args, void* stream);
 
 #ifdef __cplusplus
 }
