@@ -204,7 +204,9 @@ def load() -> ctypes.CDLL:
 
 # Order of struct Library in csrc/hbsa_host.cpp.
 _HOST_FUNCTIONS = ("hbsa_forward", "hbsa_forward_status", "hbsa_attention", "hbsa_backward", "hbsa_calculate_blocks_counted",
-                   "hbsa_calculate_blocks", "hbsa_workspace_bytes", "hbsa_backward_workspace_bytes", "hbsa_last_error")
+                   "hbsa_calculate_blocks", "hbsa_workspace_bytes", "hbsa_backward_workspace_bytes", "hbsa_last_error",
+                   "hbsa_append_to_cache", "hbsa_paged_attention", "hbsa_paged_attention_workspace_bytes", "hbsa_key_weights",
+                   "hbsa_key_weights_workspace_bytes", "hbsa_select_keys", "hbsa_compact_cache")
 
 
 def load_host(state: dict):

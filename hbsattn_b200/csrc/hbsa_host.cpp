@@ -37,6 +37,13 @@ struct Library {
   decltype(&hbsa_workspace_bytes) workspace_bytes;
   decltype(&hbsa_backward_workspace_bytes) backward_workspace_bytes;
   decltype(&hbsa_last_error) last_error;
+  decltype(&hbsa_append_to_cache) append;
+  decltype(&hbsa_paged_attention) paged;
+  decltype(&hbsa_paged_attention_workspace_bytes) paged_bytes;
+  decltype(&hbsa_key_weights) key_weights;
+  decltype(&hbsa_key_weights_workspace_bytes) key_weights_bytes;
+  decltype(&hbsa_select_keys) select;
+  decltype(&hbsa_compact_cache) compact;
 } lib = {};
 PyObject* g_state = nullptr;         // hbsa_interface._state: {"impl": ..., "last_workspace": ...}
 PyObject *s_impl = nullptr, *s_last_workspace = nullptr;
@@ -220,6 +227,11 @@ bool tracked(const at::Tensor* t) {
   if (t->unsafeGetTensorImpl()->autograd_meta() == nullptr) return false;
   return c10::GradMode::is_enabled() || t->_fw_grad(0).defined();
 }
+// The same for operators without a derivative: a view of plain tensors is no reason to go the long way.
+bool wants_gradient(const at::Tensor* t) {
+  if (t->unsafeGetTensorImpl()->autograd_meta() == nullptr) return false;
+  return (c10::GradMode::is_enabled() && t->requires_grad()) || t->_fw_grad(0).defined();
+}
 bool modes_active() { return c10::impl::TorchDispatchModeTLS::any_modes_set(); }
 
 // attention(q, k, v, cu_q, cu_k, block_mask, q_block_size, k_block_size, causal, softmax_scale[, tile_mode[, 8 tables]]) -> out
@@ -396,6 +408,283 @@ PyObject* py_calculate_blocks(PyObject*, PyObject* const* o, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ------------------------------------------------------------------------------------------------------------------
+// The paged cache: k_cache, v_cache, block_table and cache_lens of one call, checked as in paged_cache.py.
+struct CacheCall {
+  int dev = -1;
+  const at::Tensor *k, *v, *table, *lens;
+  hbsa_cache c;
+
+  const at::Tensor* int32(PyObject* o, int64_t dim) {
+    const at::Tensor* t = get_tensor(o, &dev);
+    return t && t->scalar_type() == at::kInt && t->dim() == dim ? t : nullptr;
+  }
+  // o: k_cache, v_cache, block_table, cache_lens
+  bool tensors(PyObject* const* o, bool written) {
+    k = get_tensor(o[0], &dev);
+    v = get_tensor(o[1], &dev);
+    table = int32(o[2], 2);
+    lens = int32(o[3], 1);
+    if (!k || !v || !table || !lens || k->dim() != 4 || k->sizes() != v->sizes() || k->scalar_type() != v->scalar_type() || dtype_code(k->scalar_type()) < 0) return false;
+    if (k->numel() == 0 || k->size(3) > 256 || k->size(0) > INT32_MAX || k->size(1) > INT32_MAX || k->size(2) > INT32_MAX) return false;
+    if (table->size(0) <= 0 || table->size(1) <= 0 || table->size(0) > INT32_MAX || table->stride(1) != 1 || lens->size(0) != table->size(0) || !lens->is_contiguous()) return false;
+    if (table->size(1) > INT32_MAX / k->size(1) || table->size(1) * k->size(1) >= INT32_MAX - 4095) return false;
+    if (wants_gradient(k) || wants_gradient(v) || (written && (!writable(*k) || !writable(*v)))) return false;
+    std::memset(&c, 0, sizeof(c));
+    c.k = k->data_ptr();
+    c.v = v->data_ptr();
+    for (int i = 0; i < 4; ++i) {
+      c.k_stride[i] = k->stride(i);
+      c.v_stride[i] = v->stride(i);
+    }
+    c.block_table = static_cast<const int32_t*>(table->data_ptr());
+    c.table_stride = table->stride(0);
+    c.lens = static_cast<const int32_t*>(lens->data_ptr());
+    c.num_pages = (int32_t)k->size(0);
+    c.page_size = (int32_t)k->size(1);
+    c.max_pages = (int32_t)table->size(1);
+    c.batch = (int32_t)table->size(0);
+    c.nhead_k = (int32_t)k->size(2);
+    c.headdim = (int32_t)k->size(3);
+    c.dtype = dtype_code(k->scalar_type());
+    return true;
+  }
+  static bool writable(const at::Tensor& t) {
+    for (int64_t i = 0; i < t.dim(); ++i)
+      if (t.size(i) > 1 && t.stride(i) == 0) return false;
+    return true;
+  }
+  // float32 [batch, nhead_k, >= capacity], unit stride along the last
+  const at::Tensor* weights(PyObject* o, int64_t* strides) {
+    const at::Tensor* w = get_tensor(o, &dev);
+    if (!w || w->scalar_type() != at::kFloat || w->dim() != 3 || w->size(0) != c.batch || w->size(1) != c.nhead_k || w->stride(2) != 1 || wants_gradient(w) || !writable(*w)) return nullptr;
+    if (w->size(2) < (int64_t)c.max_pages * c.page_size) return nullptr;
+    strides[0] = w->stride(0);
+    strides[1] = w->stride(1);
+    return w;
+  }
+  at::Device device() const { return at::Device(at::kCUDA, (c10::DeviceIndex)dev); }
+  at::Tensor empty(at::IntArrayRef size, at::ScalarType t) const { return at::Tensor(at::detail::empty_cuda(size, t, device(), std::nullopt)); }
+  void* stream() const { return c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream(); }
+};
+
+// Written in place: what autograd has saved of the tensor is no longer what it was.
+void touch(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
+// append(k, v, cu_seqlens, k_cache, v_cache, block_table, cache_lens) -> new lengths
+PyObject* py_append(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 7 || modes_active()) Py_RETURN_NONE;
+  CacheCall c;
+  if (!c.tensors(o + 3, true)) Py_RETURN_NONE;
+  const at::Tensor *k = get_tensor(o[0], &c.dev), *v = get_tensor(o[1], &c.dev), *cu = c.int32(o[2], 1);
+  if (!k || !v || !cu || wants_gradient(k) || wants_gradient(v) || k->dim() != 3 || k->sizes() != v->sizes() || k->size(0) > INT32_MAX || k->size(1) != c.c.nhead_k ||
+      k->size(2) != c.c.headdim || k->scalar_type() != c.k->scalar_type() || v->scalar_type() != c.k->scalar_type() || !cu->is_contiguous() || cu->size(0) != (int64_t)c.c.batch + 1)
+    Py_RETURN_NONE;
+  c10::cuda::CUDAGuard guard(c.device());
+  at::Tensor lens = c.empty({c.c.batch}, at::kInt), status = c.empty({64}, at::kByte);
+  hbsa_append_args a;
+  std::memset(&a, 0, sizeof(a));
+  a.struct_bytes = sizeof(a);
+  a.cache = c.c;
+  a.k = k->data_ptr();
+  a.v = v->data_ptr();
+  strides3(*k, a.k_stride);
+  strides3(*v, a.v_stride);
+  a.cu_seqlens = static_cast<const int32_t*>(cu->data_ptr());
+  a.new_lens = static_cast<int32_t*>(lens.data_ptr());
+  a.status = static_cast<int32_t*>(status.data_ptr());
+  a.total = (int32_t)k->size(0);
+  const int rc = lib.append(&a, c.stream());
+  if (rc != 0) {
+    fail("hbsa_append_to_cache", rc);
+    return nullptr;
+  }
+  touch(*c.k);
+  touch(*c.v);
+  if (!remember(status)) return nullptr;
+  return THPVariable_Wrap(lens);
+  END_HANDLE_TH_ERRORS
+}
+
+// paged(q, k_cache, v_cache, block_table, cache_lens, softmax_scale, block_mask, k_block_size, key_weights, return_lse) -> (out, lse | None)
+PyObject* py_paged(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 10 || modes_active()) Py_RETURN_NONE;
+  CacheCall c;
+  if (!c.tensors(o + 1, false)) Py_RETURN_NONE;
+  const at::Tensor *q = get_tensor(o[0], &c.dev), *mask = nullptr, *w = nullptr;
+  if (!q || wants_gradient(q) || q->dim() != 3 || q->scalar_type() != c.k->scalar_type() || q->size(0) != c.c.batch || q->size(2) != c.c.headdim || q->size(1) <= 0 ||
+      q->size(1) > INT32_MAX || q->size(1) % c.c.nhead_k != 0)
+    Py_RETURN_NONE;
+  hbsa_paged_attention_args a;
+  std::memset(&a, 0, sizeof(a));
+  a.struct_bytes = sizeof(a);
+  a.use_default_scale = o[5] == Py_None;
+  if (o[5] != Py_None) {
+    if (!PyFloat_CheckExact(o[5])) Py_RETURN_NONE;
+    a.softmax_scale = (float)PyFloat_AS_DOUBLE(o[5]);
+  }
+  if (o[6] != Py_None) {
+    int64_t kbs;
+    mask = get_tensor(o[6], &c.dev);
+    if (!mask || !get_int(o[7], &kbs) || mask->scalar_type() != at::kBool || mask->dim() != 3 || mask->size(0) != c.c.batch || mask->size(1) != c.c.nhead_k ||
+        kbs <= 0 || kbs % 16 != 0 || kbs > INT32_MAX || mask->size(2) > INT32_MAX || mask->size(2) * kbs < (int64_t)c.c.max_pages * c.c.page_size)
+      Py_RETURN_NONE;
+    a.block_mask = static_cast<const uint8_t*>(mask->data_ptr());
+    strides3(*mask, a.mask_stride);
+    a.num_k_block = (int32_t)mask->size(2);
+    a.k_block_size = (int32_t)kbs;
+  }
+  if (o[8] != Py_None) {
+    w = c.weights(o[8], a.weights_stride);
+    if (!w) Py_RETURN_NONE;
+    a.key_weights = static_cast<float*>(w->data_ptr());
+  }
+  const int impl = selected_impl();
+  if (impl < 0) Py_RETURN_NONE;
+  c10::cuda::CUDAGuard guard(c.device());
+  at::Tensor out = c.empty(q->sizes(), q->scalar_type()), lse;
+  if (o[9] == Py_True) lse = c.empty({q->size(0), q->size(1)}, at::kFloat);
+  a.cache = c.c;
+  a.q = q->data_ptr();
+  a.o = out.data_ptr();
+  strides3(*q, a.q_stride);
+  strides3(out, a.o_stride);
+  a.lse = lse.defined() ? static_cast<float*>(lse.data_ptr()) : nullptr;
+  a.nhead_q = (int32_t)q->size(1);
+  a.impl = impl;
+  at::Tensor ws = c.empty({(int64_t)lib.paged_bytes(&a)}, at::kByte);
+  a.workspace = ws.data_ptr();
+  a.workspace_bytes = (size_t)ws.numel();
+  const int rc = lib.paged(&a, c.stream());
+  if (rc != 0) {
+    fail("hbsa_paged_attention", rc);
+    return nullptr;
+  }
+  if (w) touch(*w);
+  if (!remember(ws)) return nullptr;
+  if (!lse.defined()) return THPVariable_Wrap(out);
+  PyObject* r = PyTuple_New(2);
+  if (!r) return nullptr;
+  PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(out));
+  PyTuple_SET_ITEM(r, 1, THPVariable_Wrap(lse));
+  return r;
+  END_HANDLE_TH_ERRORS
+}
+
+// key_weights(q, k, lse, cu_q, cu_k, block_mask, q_block_size, k_block_size, causal, softmax_scale) -> weights
+PyObject* py_key_weights(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 10 || modes_active()) Py_RETURN_NONE;
+  Call c;
+  PyObject* const data[6] = {o[0], o[1], o[1], o[3], o[4], o[5]};
+  if (!c.tensors(data) || !c.mask || c.k->size(0) == 0 || !c.options(o + 6)) Py_RETURN_NONE;
+  const at::Tensor* lse = get_tensor(o[2], &c.dev);
+  if (!lse || lse->scalar_type() != at::kFloat || lse->dim() != 2 || !lse->is_contiguous() || lse->size(0) != c.q->size(0) || lse->size(1) != c.q->size(1)) Py_RETURN_NONE;
+  if (wants_gradient(c.q) || wants_gradient(c.k) || wants_gradient(lse)) Py_RETURN_NONE;
+  const int impl = selected_impl();
+  if (impl < 0) Py_RETURN_NONE;
+  c10::cuda::CUDAGuard guard(c.device());
+  at::Tensor out = c.empty({c.k->size(0), c.k->size(1)}, at::kFloat), ws = c.workspace();
+  hbsa_key_weights_args a;
+  std::memset(&a, 0, sizeof(a));
+  a.struct_bytes = sizeof(a);
+  c.fill(impl, *c.q, ws, lse);
+  a.fwd = c.a;
+  a.weights = static_cast<float*>(out.data_ptr());
+  at::Tensor part = c.empty({(int64_t)lib.key_weights_bytes(&a)}, at::kByte);
+  a.partial_workspace = part.data_ptr();
+  a.partial_workspace_bytes = (size_t)part.numel();
+  const int rc = lib.key_weights(&a, c.stream());
+  if (rc != 0) {
+    fail("hbsa_key_weights", rc);
+    return nullptr;
+  }
+  if (!remember(ws)) return nullptr;
+  return THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
+// select(key_weights, cache_lens, budget, n_sink, n_recent) -> (kept, kept_lens)
+PyObject* py_select(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 5 || modes_active()) Py_RETURN_NONE;
+  CacheCall c;
+  int64_t budget, sink, recent;
+  const at::Tensor *w = get_tensor(o[0], &c.dev), *lens = c.int32(o[1], 1);
+  if (!w || !lens || wants_gradient(w) || !get_int(o[2], &budget) || !get_int(o[3], &sink) || !get_int(o[4], &recent)) Py_RETURN_NONE;
+  if (w->scalar_type() != at::kFloat || w->dim() != 3 || w->numel() == 0 || w->stride(2) != 1 || w->size(2) >= INT32_MAX - 4095 || w->size(0) > INT32_MAX || w->size(1) > INT32_MAX ||
+      lens->size(0) != w->size(0) || !lens->is_contiguous())
+    Py_RETURN_NONE;
+  if (budget <= 0 || sink < 0 || recent < 0 || budget > INT32_MAX || sink > budget || recent > budget || sink + recent > budget) Py_RETURN_NONE;
+  c10::cuda::CUDAGuard guard(c.device());
+  at::Tensor kept = c.empty({w->size(0), w->size(1), budget}, at::kInt), kept_lens = c.empty({w->size(0)}, at::kInt);
+  hbsa_select_keys_args a;
+  std::memset(&a, 0, sizeof(a));
+  a.struct_bytes = sizeof(a);
+  a.key_weights = static_cast<const float*>(w->data_ptr());
+  a.weights_stride[0] = w->stride(0);
+  a.weights_stride[1] = w->stride(1);
+  a.lens = static_cast<const int32_t*>(lens->data_ptr());
+  a.kept = static_cast<int32_t*>(kept.data_ptr());
+  a.kept_lens = static_cast<int32_t*>(kept_lens.data_ptr());
+  a.batch = (int32_t)w->size(0);
+  a.nhead_k = (int32_t)w->size(1);
+  a.max_len = (int32_t)w->size(2);
+  a.budget = (int32_t)budget;
+  a.n_sink = (int32_t)sink;
+  a.n_recent = (int32_t)recent;
+  const int rc = lib.select(&a, c.stream());
+  if (rc != 0) {
+    fail("hbsa_select_keys", rc);
+    return nullptr;
+  }
+  PyObject* r = PyTuple_New(2);
+  if (!r) return nullptr;
+  PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(kept));
+  PyTuple_SET_ITEM(r, 1, THPVariable_Wrap(kept_lens));
+  return r;
+  END_HANDLE_TH_ERRORS
+}
+
+// compact(k_cache, v_cache, block_table, cache_lens, kept, kept_lens, key_weights) -> True
+PyObject* py_compact(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 7 || modes_active()) Py_RETURN_NONE;
+  CacheCall c;
+  if (!c.tensors(o, true)) Py_RETURN_NONE;
+  const at::Tensor *kept = c.int32(o[4], 3), *kept_lens = c.int32(o[5], 1), *w = nullptr;
+  hbsa_compact_args a;
+  std::memset(&a, 0, sizeof(a));
+  if (o[6] != Py_None) {
+    w = c.weights(o[6], a.weights_stride);
+    if (!w) Py_RETURN_NONE;
+    a.key_weights = static_cast<float*>(w->data_ptr());
+  }
+  if (!kept || !kept_lens || !kept->is_contiguous() || !kept_lens->is_contiguous() || kept->size(0) != c.c.batch || kept->size(1) != c.c.nhead_k || kept->size(2) <= 0 ||
+      kept->size(2) > INT32_MAX || kept_lens->size(0) != c.c.batch)
+    Py_RETURN_NONE;
+  c10::cuda::CUDAGuard guard(c.device());
+  a.struct_bytes = sizeof(a);
+  a.cache = c.c;
+  a.kept = static_cast<const int32_t*>(kept->data_ptr());
+  a.kept_lens = static_cast<const int32_t*>(kept_lens->data_ptr());
+  a.budget = (int32_t)kept->size(2);
+  const int rc = lib.compact(&a, c.stream());
+  if (rc != 0) {
+    fail("hbsa_compact_cache", rc);
+    return nullptr;
+  }
+  touch(*c.k);
+  touch(*c.v);
+  if (w) touch(*w);
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
 // setup(state dict, addresses of the library's functions in the order of `Library`)
 PyObject* py_setup(PyObject*, PyObject* args) {
   PyObject *state, *addr;
@@ -417,6 +706,7 @@ PyObject* py_setup(PyObject*, PyObject* args) {
 
 #define HBSA_METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_##name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {HBSA_METHOD(attention), HBSA_METHOD(forward), HBSA_METHOD(scheduled), HBSA_METHOD(backward), HBSA_METHOD(calculate_blocks),
+                         HBSA_METHOD(append), HBSA_METHOD(paged), HBSA_METHOD(key_weights), HBSA_METHOD(select), HBSA_METHOD(compact),
                          {"setup", py_setup, METH_VARARGS, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

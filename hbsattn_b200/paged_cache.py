@@ -29,7 +29,7 @@ import torch
 from torch.autograd import forward_ad
 
 from . import _lib
-from .hbsa_interface import _DTYPES, _IMPLS, _check_csr, _prepare, _state, alloc_workspace, make_args
+from .hbsa_interface import _DTYPES, _IMPLS, _check_csr, _host, _prepare, _state, alloc_workspace, make_args
 
 
 def _refuse_gradients(name, *tensors):
@@ -65,7 +65,7 @@ def _check_cache(k_cache, v_cache, block_table, cache_lens):
 
 
 def _check_writable(name, *tensors):
-    """Tensors that are written in place: no element may be two, and none a view that autograd keeps."""
+    """Tensors that are written in place: no element may be two."""
     for t in tensors:
         assert not any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())), f"{name}: a tensor that is written to must not be expanded"
 
@@ -89,6 +89,13 @@ def _check_weights(key_weights, batch, nhead_k, capacity):
         f"key_weights must be (batch, nhead_k, at least max_pages * page_size) = ({batch}, {nhead_k}, >= {capacity})"
 
 
+def _touch(*tensors):
+    """Written in place: what autograd has saved of them is no longer what it was."""
+    for t in tensors:
+        if t is not None and not t.is_inference():
+            torch.autograd.graph.increment_version(t)
+
+
 def _run(name, args, device):
     rc = getattr(_lib.load(), name)(ctypes.byref(args), torch.cuda.current_stream(device).cuda_stream)
     if rc != 0:
@@ -99,6 +106,9 @@ def append_to_cache(k, v, cu_seqlens, k_cache, v_cache, block_table, cache_lens)
     """Writes new tokens behind those that every sequence holds already: row ``cu_seqlens[b] + i`` of ``k`` and ``v`` (packed
     ``(total, nhead_k, headdim)``, any strides) goes to position ``cache_lens[b] + i`` of sequence ``b``.  Rows outside every sequence are
     not read.  Returns the new lengths, int32 ``[batch]``; ``cache_lens`` itself is left as it is."""
+    new_lens = _host.append(k, v, cu_seqlens, k_cache, v_cache, block_table, cache_lens)     # None: what it does not take goes on here
+    if new_lens is not None:
+        return new_lens
     _same_device(k, v, cu_seqlens, k_cache, v_cache, block_table, cache_lens)
     _refuse_gradients("append_to_cache", k, v, k_cache, v_cache)
     block_table, lens = _check_cache(k_cache, v_cache, block_table, cache_lens)
@@ -121,6 +131,7 @@ def append_to_cache(k, v, cu_seqlens, k_cache, v_cache, block_table, cache_lens)
             a.k_stride[i], a.v_stride[i] = k.stride(i), v.stride(i)
         a.cu_seqlens, a.new_lens, a.status, a.total = cu.data_ptr(), new_lens.data_ptr(), status.data_ptr(), k.shape[0]
         _run("hbsa_append_to_cache", a, dev)
+        _touch(k_cache, v_cache)
         _state["last_workspace"] = status
     return new_lens
 
@@ -135,6 +146,9 @@ def paged_attention(q, k_cache, v_cache, block_table, cache_lens, softmax_scale=
     every sequence; keys of blocks that are not set are left out.  It has to cover ``max_pages * page_size`` positions.
     ``key_weights``: float32 ``(batch, nhead_k, >= max_pages * page_size)``; the attention weight of every key, summed over the q-heads of
     its kv-head, is added to it in place (what ``select_keys`` chooses by)."""
+    result = _host.paged(q, k_cache, v_cache, block_table, cache_lens, softmax_scale, block_mask, k_block_size, key_weights, bool(return_lse))
+    if result is not None:
+        return result
     _same_device(q, k_cache, v_cache, block_table, cache_lens, block_mask, key_weights)
     _refuse_gradients("paged_attention", q, k_cache, v_cache, key_weights)
     block_table, lens = _check_cache(k_cache, v_cache, block_table, cache_lens)
@@ -178,6 +192,7 @@ def paged_attention(q, k_cache, v_cache, block_table, cache_lens, softmax_scale=
             ws = torch.empty(lib.hbsa_paged_attention_workspace_bytes(ctypes.byref(a)), dtype=torch.uint8, device=dev)
             a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
             _run("hbsa_paged_attention", a, dev)
+            _touch(key_weights)
             _state["last_workspace"] = ws
     return (out, lse) if return_lse else out
 
@@ -213,6 +228,9 @@ def attention_key_weights(q, k, lse, cu_q_seqlens, cu_k_seqlens, block_mask, q_b
     rows that see the key and over the q-heads of its kv-head.  ``lse`` is what ``HBSAttention_with_lse`` has returned for the same
     arguments; rows whose ``lse`` is ``-inf`` add nothing, keys outside every sample get zeros.  The call does not wait for the device; a
     mask that contradicts the lengths gives zeros and ``last_status()`` says so, and should the kernel give up, the weights are NaN."""
+    weights = _host.key_weights(q, k, lse, cu_q_seqlens, cu_k_seqlens, block_mask, q_block_size, k_block_size, causal, softmax_scale)
+    if weights is not None:
+        return weights
     _same_device(q, k, lse, cu_q_seqlens, cu_k_seqlens, block_mask)
     _refuse_gradients("attention_key_weights", q, k, lse)
     assert block_mask.dtype == torch.bool, "block_mask must be a boolean tensor"
@@ -239,6 +257,9 @@ def select_keys(key_weights, cache_lens, budget, n_sink=0, n_recent=0):
     ``n_recent``, and of those in between the ones of the largest weight (of equal weights the lowest positions; NaN counts as the
     largest).  ``key_weights``: float32 ``(batch, nhead_k, positions)``; ``cache_lens`` are cut to its positions.  Returns ``(kept,
     kept_lens)``: int32 ``(batch, nhead_k, budget)``, ascending, ``-1`` behind the last, and int32 ``[batch]``."""
+    result = _host.select(key_weights, cache_lens, budget, n_sink, n_recent)
+    if result is not None:
+        return result
     _same_device(key_weights, cache_lens)
     _refuse_gradients("select_keys", key_weights)
     assert key_weights.dtype == torch.float32 and key_weights.ndim == 3 and key_weights.shape[2] > 0, "key_weights must be float32 (batch, nhead_k, positions)"
@@ -270,6 +291,8 @@ def compact_cache(k_cache, v_cache, block_table, cache_lens, kept, kept_lens, ke
     must belong to one sequence only; entries outside ``[0, cache_lens[b])`` move nothing.  ``key_weights`` (as for ``paged_attention``) move
     alike, and those of the positions that have become free turn zero.  ``cache_lens`` are the lengths before the move; ``kept_lens`` are
     those after it, for the calls that follow."""
+    if _host.compact(k_cache, v_cache, block_table, cache_lens, kept, kept_lens, key_weights) is not None:
+        return
     _same_device(k_cache, v_cache, block_table, cache_lens, kept, kept_lens, key_weights)
     _refuse_gradients("compact_cache", k_cache, v_cache, key_weights)
     block_table, lens = _check_cache(k_cache, v_cache, block_table, cache_lens)
@@ -294,3 +317,4 @@ def compact_cache(k_cache, v_cache, block_table, cache_lens, kept, kept_lens, ke
             a.key_weights = key_weights.data_ptr()
             a.weights_stride[0], a.weights_stride[1] = key_weights.stride(0), key_weights.stride(1)
         _run("hbsa_compact_cache", a, dev)
+        _touch(k_cache, v_cache, key_weights)

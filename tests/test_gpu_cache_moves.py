@@ -290,3 +290,29 @@ def test_compact_refusals():
         call(kept=kept.cpu())
     with pytest.raises(RuntimeError, match="derivative"):
         call(w=w.clone().requires_grad_(True))
+
+
+def test_what_autograd_has_saved_is_known_to_have_changed():
+    """The in-place operators count as in-place operators, on the native path and on the general one (odd types of the lengths)."""
+    import hbsattn_b200 as hb
+    c = make_cache(15, [64, 64], 2, 64, 16, torch.bfloat16, extra_pages=1, room=1)
+    k = torch.zeros(2, 2, 64, dtype=torch.bfloat16, device="cuda")
+    w = torch.rand(2, 2, c["table"].shape[1] * 16, device="cuda")
+    kept, n = hb.select_keys(w, c["cache_lens"], 8)
+    q = torch.zeros(2, 4, 64, dtype=torch.bfloat16, device="cuda")
+    for lens in (c["cache_lens"], c["cache_lens"].long()):
+        calls = [((c["k"], c["v"]), lambda: hb.append_to_cache(k, k, torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda"), c["k"], c["v"], c["table"], lens)),
+                 ((w,), lambda: hb.paged_attention(q, c["k"], c["v"], c["table"], lens, key_weights=w)),
+                 ((c["k"], c["v"], w), lambda: hb.compact_cache(c["k"], c["v"], c["table"], lens, kept, n, key_weights=w))]
+        for written, call in calls:
+            x = torch.ones(written[0].shape, dtype=written[0].dtype, device="cuda", requires_grad=True)
+            y = (x * written[0]).sum()
+            before = [t._version for t in written]
+            call()
+            assert all(t._version > v for t, v in zip(written, before))
+            with pytest.raises(RuntimeError, match="inplace"):
+                y.backward()
+    with torch.inference_mode():
+        held = make_cache(16, [64], 2, 64, 16, torch.bfloat16, room=1)
+        one = torch.tensor([0, 1], dtype=torch.int32, device="cuda")
+        assert hb.append_to_cache(k[:1], k[:1], one, held["k"], held["v"], held["table"], held["cache_lens"]).tolist() == [65]
