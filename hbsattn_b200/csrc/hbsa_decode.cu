@@ -3,12 +3,12 @@
 //     x_j = scale * q . k_j        o = sum_j exp(x_j - lse) v_j        lse = ln sum_j exp x_j
 // and, where wanted, weights[b, kv-head, j] += sum over the heads of the group of exp(x_j - lse).
 //
-// Up to four kernels, each started while the one before it still runs (programmatic launches):
+// Two or three kernels, each started while the one before it still runs (programmatic launches):
 //   decode_blocks   with a block mask: the list of active blocks of every (sequence, kv-head)
 //   main            one pass over K and V with the running maximum and sum of the softmax, split as hbsa_decode.cuh says
-//   decode_join     rows that several CTAs have worked on; the status words
-//   decode_weights  exp(score - lse), summed over the group, from the scores that the main kernel has left (4 bytes per key and
-//                   q-head, against 4 d bytes per key and kv-head of K and V in 16 bits): reading K again would double the traffic
+//   decode_join     rows that several CTAs have worked on; the weights: exp(score - lse), summed over the group, from the scores that the
+//                   main kernel has left (4 bytes per key and q-head, against 4 d bytes per key and kv-head of K and V in 16
+//                   bits; reading K again would add half of the traffic); the status words
 #include <string.h>
 
 #include "hbsa_decode.cuh"
@@ -39,15 +39,15 @@ __global__ void __launch_bounds__(256) decode_blocks_kernel(const __grid_constan
   int32_t* list = P.sp.list + (long long)row * P.num_k_block;
   int count = 0;
   bool last = false;
-  for (int base = 0; base < n; base += 128) {          // four loads in flight
-    bool on[4];
+  for (int base = 0; base < n; base += 512) {          // sixteen loads in flight
+    bool on[16];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 16; ++i) {
       const int j = base + 32 * i + lane;
       on[i] = j < n && m[j * P.mask_s[2]] != 0;
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 16; ++i) {
       const int j = base + 32 * i + lane;
       const uint32_t bal = __ballot_sync(0xffffffffu, on[i]);
       if (on[i]) list[count + __popc(bal & ((1u << lane) - 1u))] = j;
@@ -92,7 +92,7 @@ __global__ void __launch_bounds__(kGenThreads) decode_generic_kernel(const __gri
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (tid == 0) sh.bad = 0;
   pdl_wait();                                          // the block lists
-  decode_locate(P, blockIdx.x, P.grid, blockIdx.x == 0 ? P.sp.entry_start : nullptr, &sh.walk, sh.scratch);
+  decode_locate(P, &sh.walk, sh.scratch);
   pdl_launch();
   DecodeWalk walk = sh.walk;
   decode_fill_empty<T>(P, blockIdx.x, P.grid);
@@ -100,13 +100,12 @@ __global__ void __launch_bounds__(kGenThreads) decode_generic_kernel(const __gri
     if (P.lens[b] < 0 || P.lens[b] > P.capacity) atomicMax(&sh.bad, P.batch - b);
   const T* const K = static_cast<const T*>(P.k);
   const T* const V = static_cast<const T*>(P.v);
-  if (walk.start >= walk.end && tid == 0) P.sp.cta_start[blockIdx.x] = make_int4(-1, 0, 0, 0);
 
   // the head dimension beyond headdim stays zero
   for (int i = tid; i < kDecodeTile * KS; i += kGenThreads) sK[i] = 0.f;
   for (int i = tid; i < kDecodeTile * DP; i += kGenThreads) sV[i] = 0.f;
   for (long long t = walk.start; t < walk.end;) {
-    const DecodeRow r = decode_row_at(P, walk, t);
+    const DecodeRow r = decode_row_at(P, walk, t, blockIdx.x);
     if (t == walk.start && tid == 0) decode_note_start(P, r);
     t += r.tiles;
     const int head0 = r.hk * P.group + r.chunk * P.chunk_heads;
@@ -271,15 +270,91 @@ __global__ void __launch_bounds__(kGenThreads) decode_generic_kernel(const __gri
 }
 
 // ------------------------------------------------------------------------------------------------------------------
-// CTA (j, h): q-head h of the row whose second part is that of CTA j of the main kernel.  CTA (0, 0) writes the status words.
+// A row of the line of tiles that several runs share: its first part is that of run c0, and there are n.
+struct DecodeParts {
+  int c0, n, slot0, lanes, lane;
+  __device__ __forceinline__ DecodeParts(const DecodeCut& cut, long long row0, int row_tiles, int lanes, int lane)
+      : c0(cut.owner(row0)), n(cut.owner(row0 + row_tiles - 1) - c0 + 1), slot0(cut.first(c0) == row0 ? 0 : 1), lanes(lanes), lane(lane) {}
+  __device__ __forceinline__ long long at(int i) const { return 2ll * ((c0 + i) * lanes + lane) + (i == 0 ? slot0 : 0); }
+};
+
 constexpr int kJoinThreads = 256;
 constexpr int kJoinMost = 1024;          // CTAs of the main kernel, at most
 
+// CTA (c, y), weights: those of the keys that CTA c of the main kernel has worked on.
+__device__ __forceinline__ void add_weights(const DecodeParams& P, const DecodeCut& cut, const int4 st, int c) {
+  constexpr int WARPS = kJoinThreads / 32;
+  __shared__ float s_lse[kJoinMost];     // of the group's heads, in the log2 domain
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (st.x < 0) return;
+  DecodeWalk walk;
+  walk.start = cut.first(c / P.lanes);
+  walk.end = walk.start + cut.tiles(c / P.lanes);
+  const int hk0 = st.y / P.n_chunk, in_entry = P.mask == nullptr ? st.y : st.y % P.n_chunk;
+  walk.entry = P.mask == nullptr ? st.x : st.x * P.nhead_k + hk0;
+  walk.entry_start = walk.start - st.z - (long long)in_entry * st.w;
+  for (long long t = walk.start; t < walk.end;) {
+    const DecodeRow r = decode_row_at(P, walk, t, c);
+    const long long row0 = t - r.tile0, head0 = (long long)r.b * P.nhead_q + r.hk * P.group;
+    t += r.tiles;
+    if (r.chunk != 0) continue;          // the first chunk's tiles stand for the whole group
+    for (int h0 = 0; h0 < P.group; h0 += kJoinMost) {
+      const int heads = min(kJoinMost, P.group - h0);
+      __syncthreads();
+      for (int h = warp; h < heads; h += WARPS) {
+        const int chunk = (h0 + h) / P.chunk_heads, head = (h0 + h) % P.chunk_heads;
+        const DecodeParts parts(cut, row0 + (long long)chunk * r.row_tiles, r.row_tiles, P.lanes, c % P.lanes);
+        float lse;
+        if (parts.n == 1) {
+          lse = P.lse[head0 + h0 + h] * kDecodeLog2e;
+        } else {
+          float mx = -INFINITY, l = 0.f;
+          for (int i = lane; i < parts.n; i += 32) mx = fmaxf(mx, P.sp.part_ml[(parts.at(i) * kDecodeHeads + head) * 2]);
+#pragma unroll
+          for (int s = 16; s > 0; s >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, s));
+          const float ref = mx == -INFINITY ? 0.f : mx;
+          for (int i = lane; i < parts.n; i += 32) {
+            const float2 ml = *reinterpret_cast<const float2*>(P.sp.part_ml + (parts.at(i) * kDecodeHeads + head) * 2);
+            l += exp2f(ml.x - ref) * ml.y;
+          }
+#pragma unroll
+          for (int s = 16; s > 0; s >>= 1) l += __shfl_xor_sync(0xffffffffu, l, s);
+          lse = mx == -INFINITY && l == 0.f ? -INFINITY : mx + log2f(l);
+        }
+        if (lane == 0) s_lse[h] = lse;
+      }
+      __syncthreads();
+      const float* scores = P.sp.scores + (head0 + h0) * P.capacity;
+      float* const out = P.weights + r.b * P.weights_s[0] + r.hk * P.weights_s[1];
+      // half a tile per warp and go
+      for (int i = 2 * r.tile0 + warp; i < 2 * (r.tile0 + r.tiles); i += WARPS) {
+        int pos = i * 32 + lane;
+        if (P.mask != nullptr) {
+          const int in = pos;
+          pos = decode_piece_position(P, r, in / P.unit);
+          if (pos >= 0) pos += in % P.unit;
+        }
+        if (pos < 0 || pos >= r.len) continue;
+        float w = 0.f;
+        const float old = out[pos];
+#pragma unroll 8
+        for (int h = 0; h < heads; ++h) {
+          const float lse = s_lse[h], x = scores[(long long)h * P.capacity + pos];
+          if (lse != -INFINITY) w += exp2f(x - lse);
+        }
+        out[pos] = old + w;
+      }
+    }
+  }
+}
+
+// CTA (j, h): q-head h of the row whose second part is that of CTA j of the main kernel; behind the heads: the weights.  CTA (0, 0) writes
+// the status words.
 template <typename T>
 __global__ void __launch_bounds__(kJoinThreads) decode_join_kernel(const __grid_constant__ DecodeParams P) {
   __shared__ float s_f[kJoinMost];
   __shared__ float4 s_acc[kJoinThreads];
-  __shared__ float s_red[kJoinThreads / 32];
+  __shared__ float s_red[2][kJoinThreads / 32];
   __shared__ int s_first, s_code;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, j = blockIdx.x, head = blockIdx.y;
   if (tid == 0) {
@@ -287,7 +362,8 @@ __global__ void __launch_bounds__(kJoinThreads) decode_join_kernel(const __grid_
     s_code = 0;
   }
   pdl_wait();
-  pdl_launch();
+  const int4 st = P.sp.cta_start[j];
+  const DecodeCut cut(*P.sp.total, P.runs);
   __syncthreads();
   for (int c = tid; c < P.grid; c += kJoinThreads) {
     const int code = P.sp.cta_status[2 * c];
@@ -313,109 +389,72 @@ __global__ void __launch_bounds__(kJoinThreads) decode_join_kernel(const __grid_
     }
     return;
   }
-  if (j == 0) return;
-  const int4 st = P.sp.cta_start[j];
-  const long long total = P.sp.entry_start[P.entries];
+  if (head == P.chunk_heads) {
+    add_weights(P, cut, st, j);
+    return;
+  }
   if (st.x < 0 || st.z == 0) return;
-  const int hk = st.y / P.n_chunk, chunk = st.y % P.n_chunk;
+  const int run = j / P.lanes, hk = st.y / P.n_chunk * P.lanes + j % P.lanes, chunk = st.y % P.n_chunk;
   if (head >= min(P.chunk_heads, P.group - chunk * P.chunk_heads)) return;
-  const long long row0 = decode_first(j, total, P.grid) - st.z;
-  const int c0 = decode_owner(row0, total, P.grid), n = decode_owner(row0 + st.w - 1, total, P.grid) - c0 + 1;
-  if (j != decode_owner(decode_first(c0 + 1, total, P.grid), total, P.grid)) return;      // not the row's second CTA with tiles
-  const int slot0 = decode_first(c0, total, P.grid) == row0 ? 0 : 1;
-  auto part_of = [&](int i) -> long long { return 2ll * (c0 + i) + (i == 0 ? slot0 : 0); };
-  auto there = [&](int i) { return decode_first(c0 + i, total, P.grid) < decode_first(c0 + i + 1, total, P.grid); };
+  const DecodeParts parts(cut, cut.first(run) - st.z, st.w, P.lanes, j % P.lanes);
+  if (run != parts.c0 + 1) return;
+  const int n = parts.n;
 
+  // the outputs of the first parts are on their way while the factors are made
+  const int quads = P.d_pad / 4, groups = kJoinThreads / quads, quad = tid % quads, g = tid / quads;
+  auto part_of = [&](int i) { return *reinterpret_cast<const float4*>(P.sp.part_o + (parts.at(i) * kDecodeHeads + head) * P.d_pad + quad * 4); };
+  constexpr int AHEAD = 4;
+  float4 early[AHEAD];
+#pragma unroll
+  for (int e = 0; e < AHEAD; ++e) early[e] = g + e * groups < n ? part_of(g + e * groups) : make_float4(0.f, 0.f, 0.f, 0.f);
+  auto ml_of = [&](int i) { return *reinterpret_cast<const float2*>(P.sp.part_ml + (parts.at(i) * kDecodeHeads + head) * 2); };
   float mx = -INFINITY;
-  for (int i = tid; i < n; i += kJoinThreads)
-    if (there(i)) mx = fmaxf(mx, P.sp.part_ml[(part_of(i) * kDecodeHeads + head) * 2]);
+  float2 first = make_float2(-INFINITY, 0.f);
+  if (tid < n) first = ml_of(tid);
+  for (int i = tid; i < n; i += kJoinThreads) mx = fmaxf(mx, i == tid ? first.x : ml_of(i).x);
 #pragma unroll
   for (int s = 16; s > 0; s >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, s));
-  if (lane == 0) s_red[warp] = mx;
+  if (lane == 0) s_red[0][warp] = mx;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kJoinThreads / 32; ++w) mx = fmaxf(mx, s_red[w]);
+  for (int w = 0; w < kJoinThreads / 32; ++w) mx = fmaxf(mx, s_red[0][w]);
   const float ref = mx == -INFINITY ? 0.f : mx;
   float l = 0.f;
   for (int i = tid; i < n; i += kJoinThreads) {
-    float f = 0.f;
-    if (there(i)) {
-      const float2 ml = *reinterpret_cast<const float2*>(P.sp.part_ml + (part_of(i) * kDecodeHeads + head) * 2);
-      f = exp2f(ml.x - ref);
-      l += f * ml.y;
-    }
+    const float2 ml = i == tid ? first : ml_of(i);
+    const float f = exp2f(ml.x - ref);
+    l += f * ml.y;
     s_f[i] = f;
   }
 #pragma unroll
   for (int s = 16; s > 0; s >>= 1) l += __shfl_xor_sync(0xffffffffu, l, s);
-  __syncthreads();
-  if (lane == 0) s_red[warp] = l;
+  if (lane == 0) s_red[1][warp] = l;
   __syncthreads();
   l = 0.f;
 #pragma unroll
-  for (int w = 0; w < kJoinThreads / 32; ++w) l += s_red[w];
-  const int quads = P.d_pad / 4, groups = kJoinThreads / quads, quad = tid % quads;
+  for (int w = 0; w < kJoinThreads / 32; ++w) l += s_red[1][w];
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (int i = tid / quads; i < n; i += groups) {
-    if (!there(i)) continue;
-    const float f = s_f[i];
-    const float4 x = *reinterpret_cast<const float4*>(P.sp.part_o + (part_of(i) * kDecodeHeads + head) * P.d_pad + quad * 4);
+  auto add = [&](float f, const float4 x) {
     acc.x = fmaf(f, x.x, acc.x);
     acc.y = fmaf(f, x.y, acc.y);
     acc.z = fmaf(f, x.z, acc.z);
     acc.w = fmaf(f, x.w, acc.w);
-  }
+  };
+#pragma unroll
+  for (int e = 0; e < AHEAD; ++e)
+    if (g + e * groups < n) add(s_f[g + e * groups], early[e]);
+#pragma unroll 4
+  for (int i = g + AHEAD * groups; i < n; i += groups) add(s_f[i], part_of(i));
   s_acc[tid] = acc;
   __syncthreads();
   const bool none = mx == -INFINITY && l == 0.f;
   const int hq = hk * P.group + chunk * P.chunk_heads + head;
   if (tid < P.headdim) {
     float x = 0.f;
-    for (int g = 0; g < groups; ++g) x += reinterpret_cast<const float*>(s_acc)[g * P.d_pad + tid];
+    for (int i = 0; i < groups; ++i) x += reinterpret_cast<const float*>(s_acc)[i * P.d_pad + tid];
     static_cast<T*>(P.o)[st.x * P.o_s[0] + hq * P.o_s[1] + tid * P.o_s[2]] = from_f<T>(none ? 0.f : x / l);
   }
   if (tid == 0 && P.lse != nullptr) P.lse[(long long)st.x * P.nhead_q + hq] = none ? -INFINITY : (mx + log2f(l)) * kDecodeLn2;
-}
-
-// ------------------------------------------------------------------------------------------------------------------
-// Every warp takes tiles of the line of tiles, one at a time, and adds the weights of their 64 keys.
-constexpr int kWeightsThreads = 256;
-
-__global__ void __launch_bounds__(kWeightsThreads) decode_weights_kernel(const __grid_constant__ DecodeParams P) {
-  __shared__ DecodeWalk s_walk;
-  __shared__ long long s_scratch[kWeightsThreads / 32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  pdl_wait();
-  if (P.sp.status[0] == HBSA_STATUS_WAIT_LIMIT) return;
-  decode_locate(P, blockIdx.x, gridDim.x, nullptr, &s_walk, s_scratch);
-  DecodeWalk walk = s_walk;
-  for (long long t = walk.start; t < walk.end;) {
-    const DecodeRow r = decode_row_at(P, walk, t);
-    t += r.tiles;
-    if (r.chunk != 0) continue;          // the first chunk's tiles stand for the whole group
-    for (int tile = r.tile0 + warp; tile < r.tile0 + r.tiles; tile += kWeightsThreads / 32) {
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int in = half * 32 + lane;
-        int pos = tile * kDecodeTile + in;
-        if (P.mask != nullptr) {
-          pos = decode_piece_position(P, r, pos / P.unit);
-          if (pos >= 0) pos += in % P.unit;
-        }
-        if (pos < 0 || pos >= r.len) continue;
-        const long long row = (long long)r.b * P.nhead_q + r.hk * P.group;
-        float w = 0.f;
-#pragma unroll 4
-        for (int h = 0; h < P.group; ++h) {
-          const float lse = P.lse[row + h];
-          const float x = P.sp.scores[(row + h) * P.capacity + pos];
-          if (lse != -INFINITY) w += exp2f(x - lse * kDecodeLog2e);
-        }
-        P.weights[r.b * P.weights_s[0] + r.hk * P.weights_s[1] + pos] += w;
-      }
-    }
-  }
 }
 
 template <typename T, int DP, int VEC>
@@ -460,7 +499,7 @@ size_t carve_decode(const DecodeParams& P, char* base, DecodeSpace* s, bool own_
   s->status = reinterpret_cast<int32_t*>(take(kStatusWords * 4));
   s->cta_status = reinterpret_cast<int32_t*>(take((size_t)P.grid * 8));
   s->cta_start = reinterpret_cast<int4*>(take((size_t)P.grid * 16));
-  s->entry_start = reinterpret_cast<long long*>(take(((size_t)P.entries + 1) * 8));
+  s->total = reinterpret_cast<long long*>(take(8));
   s->pieces = reinterpret_cast<int32_t*>(take(P.mask ? rows * 4 : 0));
   s->list = reinterpret_cast<int32_t*>(take(P.mask ? rows * P.num_k_block * 4 : 0));
   s->lse = reinterpret_cast<float*>(take(own_lse ? heads * 4 : 0));
@@ -520,8 +559,6 @@ int make_decode(const hbsa_paged_attention_args* a, bool need_tensors, DecodePar
   P->group = a->nhead_q / c.nhead_k;
   P->headdim = c.headdim;
   P->d_pad = c.headdim <= 64 ? 64 : c.headdim <= 128 ? 128 : 256;
-  P->n_chunk = (P->group + kDecodeHeads - 1) / kDecodeHeads;
-  P->chunk_heads = (P->group + P->n_chunk - 1) / P->n_chunk;
   P->kbs = a->k_block_size;
   P->num_k_block = a->num_k_block;
   P->entries = a->block_mask ? c.batch * c.nhead_k : c.batch;
@@ -532,11 +569,17 @@ int make_decode(const hbsa_paged_attention_args* a, bool need_tensors, DecodePar
   const char* why = decode_sm100_ineligible_reason(*a, scale);
   if (need_tensors && a->impl == HBSA_IMPL_SM100 && why) return set_last_error("the tensor-core kernel cannot run this problem: %s", why), HBSA_ERR_UNSUPPORTED;
   *sm100 = !why && a->impl != HBSA_IMPL_GENERIC;
+  const int most_heads = *sm100 && P->d_pad == 256 ? 16 : kDecodeHeads;
+  P->n_chunk = (P->group + most_heads - 1) / most_heads;
+  P->chunk_heads = (P->group + P->n_chunk - 1) / P->n_chunk;
   P->unit = kDecodeTile;
   if (*sm100) P->unit = gcd(P->unit, P->page);
   if (P->mask) P->unit = gcd(P->unit, P->kbs);
   P->pieces_per_block = P->mask ? P->kbs / P->unit : 0;
-  P->grid = decode_grid(*sm100, P->d_pad);
+  P->one_box = P->headdim % 64 == 0;
+  P->lanes = P->mask || P->nhead_k % 2 ? 1 : P->nhead_k % 4 ? 2 : 4;
+  P->runs = decode_grid(*sm100, P->d_pad) / P->lanes;
+  P->grid = P->runs * P->lanes;
   const bool own_lse = a->key_weights && !a->lse;
   *bytes = carve_decode(*P, static_cast<char*>(a->workspace), &P->sp, own_lse);
   P->lse = own_lse ? P->sp.lse : a->lse;
@@ -589,14 +632,12 @@ int hbsa_paged_attention(const hbsa_paged_attention_args* args, void* stream_) {
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)P.grid, (unsigned)P.chunk_heads);
+  cfg.gridDim = dim3((unsigned)P.grid, (unsigned)(P.chunk_heads + (P.weights ? 1 : 0)));
   cfg.blockDim = dim3(hbsa::kJoinThreads);
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   if ((e = cudaLaunchKernelEx(&cfg, join, P)) != cudaSuccess) return failed(e);
-  if (P.weights && (e = hbsa::launch_kernel(hbsa::decode_weights_kernel, (unsigned)(4 * hbsa::sm100_sm_count()), hbsa::kWeightsThreads, 0, true, stream, P)) != cudaSuccess)
-    return failed(e);
   return 0;
 }
 

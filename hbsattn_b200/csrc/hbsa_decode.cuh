@@ -3,9 +3,11 @@
 //
 // One row = one (sequence, kv-head, chunk of at most 32 q-heads of its group).  A row's keys come in tiles of 64; without a
 // block mask tile i holds positions 64 i .. 64 i + 63, with one the tile is strung together from pieces of `unit` positions of the
-// active blocks.  The tiles of all rows stand in one line (sequence, kv-head, chunk, tile), and CTA c of G takes the tiles
-// [c T / G, (c + 1) T / G): every CTA reads the same number of keys, whatever the lengths are, and at most its first and its
-// last row are shared with neighbours.  Those leave (maximum, sum, unnormalised output) in two slots of the CTA's own, which the
+// active blocks.  The tiles of all rows stand in one line (sequence, kv-head, chunk, tile), which is cut into runs of the same
+// length, up to one tile: every CTA reads the same number of keys, whatever the lengths are, and at most its first and its
+// last row are shared with neighbours.  Without a mask `lanes` (1, 2 or 4) neighbouring kv-heads are worked on side by side: the line holds
+// every lanes-th kv-head, and the CTAs lanes * c .. take run c of it, one kv-head each, so that what lies together in memory is
+// read at the same time (16 x 24576 keys, 8 heads of 64 inside the slots: 160 us with one lane).  Those leave (maximum, sum, unnormalised output) in two slots of the CTA's own, which the
 // join kernel puts together in the order of the CTAs, so that results do not depend on timing.
 #pragma once
 #include "hbsa_common.cuh"
@@ -21,8 +23,8 @@ constexpr float kDecodeLn2 = 0.6931471805599453f;
 struct DecodeSpace {
   int32_t* status;           // [kStatusWords], written by the join kernel
   int32_t* cta_status;       // [G][2] what CTA c has to report: HBSA_STATUS_*, sequence
-  int4* cta_start;           // [G] {row's sequence, kv-head * n_chunk + chunk, tiles of the row before the CTA's first, tiles of the row}
-  long long* entry_start;    // [entries + 1] first tile of every entry (a sequence, or a (sequence, kv-head) where there is a mask)
+  int4* cta_start;           // [G] of the CTA's first row {sequence, kv-head / lanes * n_chunk + chunk, its tiles before the CTA's first, its tiles}
+  long long* total;          // [1] tiles of the line
   int32_t* pieces;           // [batch * nhead_k] pieces of the active blocks (mask)
   int32_t* list;             // [batch * nhead_k][num_k_block] the active blocks, ascending (mask)
   float* lse;                // [batch, nhead_q] (weights, where the caller wants no lse)
@@ -48,16 +50,27 @@ struct DecodeParams {
   int n_chunk, chunk_heads;  // chunks of a group, q-heads of every chunk but perhaps the last
   int kbs, num_k_block;
   int unit, pieces_per_block;
+  int one_box;               // tensor-core kernel: one copy brings all columns of a piece
   int entries;
   float scale_log2;
   long long wait_budget;
   int debug_stall;
-  int grid;                  // G
+  int grid, lanes, runs;     // G = lanes * runs
 };
 
-// First tile of CTA c, and the CTA that owns tile t (the last c whose first tile is not behind t; it is never an empty one).
-__device__ __forceinline__ long long decode_first(long long c, long long total, int grid) { return c * total / grid; }
-__device__ __forceinline__ int decode_owner(long long t, long long total, int grid) { return (int)(((t + 1) * grid - 1) / total); }
+// The cut of `total` tiles into `grid` runs: the first `rem` have base + 1 tiles, the others base.
+struct DecodeCut {
+  long long base;
+  int rem;
+  __device__ __forceinline__ DecodeCut(long long total, int grid) : base(total / grid), rem((int)(total - total / grid * grid)) {}
+  __device__ __forceinline__ long long first(int c) const { return c * base + min(c, rem); }
+  __device__ __forceinline__ int tiles(int c) const { return (int)base + (c < rem ? 1 : 0); }
+  // the run that has tile t
+  __device__ __forceinline__ int owner(long long t) const {
+    const long long front = rem * (base + 1);
+    return t < front ? (int)(t / (base + 1)) : rem + (int)((t - front) / base);
+  }
+};
 
 __device__ __forceinline__ int decode_len(const DecodeParams& P, int b) { return max(0, min(P.lens[b], P.capacity)); }
 // Tiles of one row of entry e.
@@ -65,7 +78,7 @@ __device__ __forceinline__ int decode_row_tiles(const DecodeParams& P, int e) {
   if (P.mask == nullptr) return (decode_len(P, e) + kDecodeTile - 1) / kDecodeTile;
   return (int)(((long long)P.sp.pieces[e] * P.unit + kDecodeTile - 1) / kDecodeTile);
 }
-__device__ __forceinline__ int decode_entry_rows(const DecodeParams& P) { return P.mask == nullptr ? P.nhead_k * P.n_chunk : P.n_chunk; }
+__device__ __forceinline__ int decode_entry_rows(const DecodeParams& P) { return P.mask == nullptr ? P.nhead_k / P.lanes * P.n_chunk : P.n_chunk; }
 
 // One row, and the tiles of it that a CTA works on.
 struct DecodeRow {
@@ -75,16 +88,16 @@ struct DecodeRow {
   int len, pieces, entry;
 };
 
-// Finds the place of the tile line at which a CTA starts; all threads of the block call it.  `walk` (shared) receives the entry
-// that holds `first(total)` and the entry's first tile; returns the total.  `table`: the entries' first tiles go there too.
+// A place on the line of tiles: the entry (a sequence, or a (sequence, kv-head) where there is a mask) and its first tile.
 struct DecodeWalk {
-  long long total, start, end, entry_start;
+  long long start, end, entry_start;
   int entry;
 };
-__device__ __forceinline__ void decode_locate(const DecodeParams& P, int cta, int grid, long long* table, DecodeWalk* walk, long long* scratch) {
+// Finds the place at which a CTA's run starts; all threads of the block call it.  `scratch`: shared, one word per warp.
+__device__ __forceinline__ void decode_locate(const DecodeParams& P, DecodeWalk* walk, long long* scratch) {
   const int tid = threadIdx.x, n_threads = blockDim.x, lane = tid & 31, warp = tid >> 5, n_warps = (n_threads + 31) >> 5;
   const int rows = decode_entry_rows(P);
-  const int e0 = (int)((long long)P.entries * tid / n_threads), e1 = (int)((long long)P.entries * (tid + 1) / n_threads);
+  const int per = (P.entries + n_threads - 1) / n_threads, e0 = min(per * tid, P.entries), e1 = min(e0 + per, P.entries);
   long long sum = 0;
   for (int e = e0; e < e1; ++e) sum += (long long)decode_row_tiles(P, e) * rows;
   long long incl = sum;
@@ -101,22 +114,20 @@ __device__ __forceinline__ void decode_locate(const DecodeParams& P, int cta, in
     total += scratch[w];
   }
   before += incl - sum;
-  const long long start = decode_first(cta, total, grid), end = decode_first(cta + 1, total, grid);
+  const DecodeCut cut(total, P.runs);
+  const int run = blockIdx.x / P.lanes;
+  const long long start = cut.first(run), end = start + cut.tiles(run);
   if (tid == 0) {
-    walk->total = total;
     walk->start = start;
     walk->end = end;
-    walk->entry = P.entries;
-    walk->entry_start = total;
-    if (table != nullptr) table[P.entries] = total;
+    if (blockIdx.x == 0) *P.sp.total = total;
+    if (start == end) P.sp.cta_start[blockIdx.x] = make_int4(-1, 0, 0, 0);
   }
-  __syncthreads();
-  if (table != nullptr || (start < end && start >= before && start < before + sum)) {
+  if (start < end && start >= before && start < before + sum) {
     long long at = before;
     for (int e = e0; e < e1; ++e) {
-      if (table != nullptr) table[e] = at;
       const long long n = (long long)decode_row_tiles(P, e) * rows;
-      if (start < end && start >= at && start < at + n) {
+      if (start >= at && start < at + n) {
         walk->entry = e;
         walk->entry_start = at;
       }
@@ -126,8 +137,8 @@ __device__ __forceinline__ void decode_locate(const DecodeParams& P, int cta, in
   __syncthreads();
 }
 
-// The row that holds tile t, and as much of it as lies before `end`; moves `walk` on to the row's entry.
-__device__ __forceinline__ DecodeRow decode_row_at(const DecodeParams& P, DecodeWalk& walk, long long t) {
+// The row of CTA `cta` that holds tile t, and as much of it as lies before `end`; moves `walk` on to the row's entry.
+__device__ __forceinline__ DecodeRow decode_row_at(const DecodeParams& P, DecodeWalk& walk, long long t, int cta) {
   DecodeRow r;
   const int rows = decode_entry_rows(P);
   int tiles = decode_row_tiles(P, walk.entry);
@@ -139,9 +150,8 @@ __device__ __forceinline__ DecodeRow decode_row_at(const DecodeParams& P, Decode
   const long long row0 = walk.entry_start + (long long)in_entry * tiles;
   r.entry = walk.entry;
   r.b = P.mask == nullptr ? walk.entry : walk.entry / P.nhead_k;
-  const int hc = P.mask == nullptr ? in_entry : walk.entry % P.nhead_k * P.n_chunk + in_entry;
-  r.hk = hc / P.n_chunk;
-  r.chunk = hc % P.n_chunk;
+  r.hk = P.mask == nullptr ? in_entry / P.n_chunk * P.lanes + cta % P.lanes : walk.entry % P.nhead_k;
+  r.chunk = in_entry % P.n_chunk;
   r.row_tiles = tiles;
   r.tile0 = (int)(t - row0);
   r.tiles = (int)(min(walk.end, row0 + tiles) - t);
@@ -173,7 +183,7 @@ __device__ __forceinline__ void decode_fill_empty(const DecodeParams& P, int cta
 
 // What every CTA of the main kernel writes down for the join: its first row.
 __device__ __forceinline__ void decode_note_start(const DecodeParams& P, const DecodeRow& r) {
-  P.sp.cta_start[blockIdx.x] = make_int4(r.b, r.hk * P.n_chunk + r.chunk, r.tile0, r.row_tiles);
+  P.sp.cta_start[blockIdx.x] = make_int4(r.b, r.hk / P.lanes * P.n_chunk + r.chunk, r.tile0, r.row_tiles);
 }
 
 __device__ __forceinline__ void decode_note_status(const DecodeParams& P, int status, int sequence) {

@@ -6,12 +6,15 @@
 // works on 128 rows, of which a GQA group fills 1 to 32, and its softmax would have to go through tensor memory and back, while
 // a warp here keeps scores, statistics and output in registers and meets no other warp before the row ends.
 //
-// 288 threads, one persistent CTA per SM:
-//   warp 8      walks the CTA's rows, looks the pages up 32 pieces at a time (the next 32 while these are issued) and loads K and V tiles
-//               of 64 keys by TMA, 128-byte swizzled, into a ring of as many stages as fit: one box per panel of 64 columns
-//               and piece; a piece is the largest power of two up to 64 positions that neither a page nor a block of the mask cuts.
-//   warps 0-7   warp w takes keys 16 (w mod 4) .. + 15 of a tile: S = Q K^T (16 heads x 16 keys), running maximum and sum, O += P V.  With up
-//               to 16 heads warps 0-3 take the even tiles and 4-7 the odd ones, with up to 32 both take every tile, 16 heads each.
+// 320 threads, one persistent CTA per SM:
+//   warps 8, 9  walk the CTA's rows, look the pages up 32 pieces at a time (the next 32 while these are issued) and load K (warp 8) and
+//               V (warp 9) by TMA, 128-byte swizzled, into a ring of as many stages as fit; a stage is one or two tiles of 64 keys.  A piece
+//               is the largest power of two up to 64 positions that neither a page nor a block of the mask cuts; one box brings
+//               all of its columns where headdim is a multiple of 64 (x, slot, panel), one per panel of 64 columns otherwise.
+//   warps 0-7   warp w takes a slab of 16 or 32 keys of a stage, the (w mod 4)-th: S = Q K^T (16 heads), running maximum and sum, O += P V.
+//               With up to 16 heads warps 0-3 take the even stages and 4-7 the odd ones, with up to 32 both take every stage, 16
+//               heads each.  256 columns of O do not fit a warp's registers: there both take every stage, up to 16 heads and half
+//               of O's columns each (the scores are made twice), and Q is read from shared memory for every product.
 // At the end of a row the warps' parts are put together through shared memory, 64 columns at a time.
 // Positions behind the length share the last tile with others and may hold anything: their scores are set to -inf, and their
 // rows of V to zero in shared memory (0 x NaN would come out of the product otherwise).
@@ -24,38 +27,45 @@ namespace hbsa {
 
 namespace {
 
-constexpr int kThreads = 288;
+constexpr int kThreads = 320;
 constexpr int kConsumers = 8;
-constexpr int kSlabs = 4;                // slabs of 16 keys in a tile
+constexpr int kSlabs = 4;                // slabs of a stage
 constexpr int kRowSlots = 2;
 
-template <int D> struct Ring { static constexpr int kStages = D == 64 ? 12 : D == 128 ? 6 : 3; };
-
-struct SlabInfo {
-  int pos;               // position of the slab's first key
-  int n;                 // keys of it that take part
-  int hidden;            // keys below the length on a page that does not exist
+// Per head dimension of the tiles: keys of a slab in units of 16, stages, columns of O of a warp.
+template <int D> struct Shape {
+  static constexpr int kUnits = D == 64 ? 2 : 1;
+  static constexpr int kStages = D == 256 ? 3 : 6;
+  static constexpr int kKeys = kSlabs * kUnits * 16;             // of a stage
+  static constexpr bool kHalves = D == 256;                      // warps w and w + 4 share the columns of O
+  static constexpr int kColumns = kHalves ? D / 2 : D;
 };
 
-template <int STAGES> struct __align__(16) DecodeControl {
-  unsigned long long full[STAGES], free[STAGES];
+struct __align__(16) SlabInfo {          // of 16 keys
+  int pos;               // position of the first key
+  int n;                 // keys that take part
+  int hidden;            // keys below the length on a page that does not exist
+  int pad;
+};
+
+template <int D> struct __align__(16) DecodeControl {
+  SlabInfo slab[Shape<D>::kStages][kSlabs * Shape<D>::kUnits];
+  unsigned long long full[Shape<D>::kStages], free[Shape<D>::kStages];
   unsigned long long row_full[kRowSlots], row_done[kRowSlots], meet;
   DecodeWalk walk;
   long long scratch[16];
   DecodeRow row[kRowSlots];
-  SlabInfo slab[STAGES][kSlabs];
   float ml[kConsumers][16][2];
   int abort_flag, bad;
 };
 
-template <int D> constexpr size_t decode_smem() {
-  return (size_t)Ring<D>::kStages * 2 * kDecodeTile * D * 2 + kConsumers * 16 * 64 * 4 + sizeof(DecodeControl<Ring<D>::kStages>);
-}
+constexpr uint32_t kPartBytes = kConsumers * 16 * 64 * 4;
+template <int D> constexpr size_t decode_smem() { return (size_t)Shape<D>::kStages * 2 * Shape<D>::kKeys * D * 2 + kPartBytes + sizeof(DecodeControl<D>); }
 static_assert(decode_smem<64>() <= 227 * 1024 && decode_smem<128>() <= 227 * 1024 && decode_smem<256>() <= 227 * 1024, "shared memory of one CTA");
 
-__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2, int c3) {
-  asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
-               ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+__device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2, int c3, int c4) {
+  asm volatile("cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
+               ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4)
                : "memory");
 }
 __device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
@@ -73,12 +83,18 @@ template <bool BF16> __device__ __forceinline__ void mma16816(float (&c)[4], con
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// A wait of a whole warp that usually finds the phase complete.
+__device__ __forceinline__ bool quick_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, long long budget) {
+  if (__all_sync(0xffffffffu, ptx::mbar_test(bar, parity))) return true;
+  const bool ok = warp_wait(bar, parity, abort_flag, budget);
+  __syncwarp();
+  return ok;
+}
 // The consumer warps meet; false when one of them has given up (a named barrier would wait for it for good).
 __device__ __forceinline__ bool meet(uint32_t bar, uint32_t& par, volatile int* abort_flag, long long budget) {
   __syncwarp();
   if ((threadIdx.x & 31) == 0) ptx::mbar_arrive(bar);
-  const bool ok = warp_wait(bar, par, abort_flag, budget);
-  __syncwarp();
+  const bool ok = quick_wait(bar, par, abort_flag, budget);
   par ^= 1u;
   return ok;
 }
@@ -87,65 +103,68 @@ template <int D, bool BF16>
 __global__ void __launch_bounds__(kThreads, 1)
 decode_sm100_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ DecodeParams P) {
   using namespace ptx;
-  constexpr int STAGES = Ring<D>::kStages, PANELS = D / 64, KSTEPS = D / 16;
-  constexpr uint32_t PANEL = kDecodeTile * 128u, HALF = PANEL * PANELS, STAGE = 2 * HALF;       // bytes: 64 rows of 128, K or V, both
+  constexpr int STAGES = Shape<D>::kStages, UNITS = Shape<D>::kUnits, PANELS = D / 64, KSTEPS = D / 16;
+  constexpr uint32_t HALF = (uint32_t)Shape<D>::kKeys * D * 2u, STAGE = 2 * HALF;      // bytes of K or V, and of both
+  constexpr bool HALVES = Shape<D>::kHalves;
+  constexpr int COLUMNS = Shape<D>::kColumns;
   using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
   extern __shared__ __align__(1024) uint8_t base[];  // 1024-byte aligned tiles for the 128-byte swizzle
   const uint32_t ring = smem_u32(base);
-  float* const part = reinterpret_cast<float*>(base + STAGES * STAGE);                           // [kConsumers][16][64]
-  auto* const ctl = reinterpret_cast<DecodeControl<STAGES>*>(base + STAGES * STAGE + kConsumers * 16 * 64 * 4);
+  float* const part = reinterpret_cast<float*>(base + STAGES * STAGE);                 // [kConsumers][16][64]
+  auto* const ctl = reinterpret_cast<DecodeControl<D>*>(base + STAGES * STAGE + kPartBytes);
   volatile int* const abort_flag = &ctl->abort_flag;
   const long long budget = P.wait_budget;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t b_full = smem_u32(ctl->full), b_free = smem_u32(ctl->free), b_row_full = smem_u32(ctl->row_full), b_row_done = smem_u32(ctl->row_done);
-  const bool wide = P.chunk_heads > 16;            // every tile goes to all eight warps
+  const bool wide = !HALVES && P.chunk_heads > 16; // two times 16 heads
+  const bool all = HALVES || wide;                 // every stage goes to all eight warps
+  const uint32_t piece_panel = (uint32_t)P.unit * 128u;                                // bytes of a piece's panel of 64 columns
   if (tid == 0) {
     for (int i = 0; i < STAGES; ++i) {
-      mbar_init(b_full + 8 * i, 1);
-      mbar_init(b_free + 8 * i, wide ? kConsumers : kSlabs);
+      mbar_init(b_full + 8 * i, 2);
+      mbar_init(b_free + 8 * i, all ? kConsumers : kSlabs);
     }
     for (int i = 0; i < kRowSlots; ++i) {
       mbar_init(b_row_full + 8 * i, 1);
       mbar_init(b_row_done + 8 * i, kConsumers);
     }
+    mbar_init(smem_u32(&ctl->meet), kConsumers);
     ctl->abort_flag = (ring & 1023u) != 0 ? 1 : 0;
     ctl->bad = 0;
-    mbar_init(smem_u32(&ctl->meet), kConsumers);
     fence_barrier_init();
   }
-  if (tid == kThreads - 32) {
-    prefetch_tensormap(&tm_k);
-    prefetch_tensormap(&tm_v);
-  }
+  if (tid == kConsumers * 32) prefetch_tensormap(&tm_k);
+  if (tid == kConsumers * 32 + 32) prefetch_tensormap(&tm_v);
   pdl_wait();                                      // the block lists
-  decode_locate(P, blockIdx.x, P.grid, blockIdx.x == 0 ? P.sp.entry_start : nullptr, &ctl->walk, ctl->scratch);
+  decode_locate(P, &ctl->walk, ctl->scratch);
   pdl_launch();
 
-  if (warp == kConsumers) {
-    // =============================== rows, pages, TMA ===============================
+  if (warp >= kConsumers) {
+    // =============================== rows, pages, TMA: K in the first of the two warps, V in the second ===============================
+    const bool first_warp = warp == kConsumers;
+    const CUtensorMap* const map = first_warp ? &tm_k : &tm_v;
     DecodeWalk walk = ctl->walk;
-    if (walk.start >= walk.end && lane == 0) P.sp.cta_start[blockIdx.x] = make_int4(-1, 0, 0, 0);
     bool ok = *abort_flag == 0 && P.debug_stall == 0;
     int stage = 0, n_rows = 0, used = 0;
     uint32_t par = 1u;
-    const int per_tile = kDecodeTile / P.unit;                 // pieces of a tile: 1, 2 or 4
-    const uint32_t piece_bytes = (uint32_t)P.unit * 128u;
+    const int per_tile = kDecodeTile / P.unit, per_stage = Shape<D>::kKeys / P.unit;    // pieces; per_stage <= 8
     for (long long t = walk.start; ok;) {
-      if (n_rows >= kRowSlots) ok = warp_wait(b_row_done + 8 * (n_rows & 1), (uint32_t)((n_rows >> 1) - 1) & 1u, abort_flag, budget);
-      if (!ok) break;
       DecodeRow r;
       r.b = -1;
-      if (t < walk.end) r = decode_row_at(P, walk, t);
-      if (lane == 0) {
-        ctl->row[n_rows & 1] = r;
-        if (r.b >= 0 && t == walk.start) decode_note_start(P, r);
-        __threadfence_block();
-        mbar_arrive(b_row_full + 8 * (n_rows & 1));
+      if (t < walk.end) r = decode_row_at(P, walk, t, blockIdx.x);
+      if (first_warp) {
+        if (n_rows >= kRowSlots) ok = warp_wait(b_row_done + 8 * (n_rows & 1), (uint32_t)((n_rows >> 1) - 1) & 1u, abort_flag, budget);
+        if (!ok) break;
+        if (lane == 0) {
+          ctl->row[n_rows & 1] = r;
+          if (r.b >= 0 && t == walk.start) decode_note_start(P, r);
+          mbar_arrive(b_row_full + 8 * (n_rows & 1));
+        }
+        ++n_rows;
       }
-      ++n_rows;
       if (r.b < 0) break;
       t += r.tiles;
-      // lane i: position and page of piece first + i of the row; page -1: there is none
+      // lane i: position and page of piece first + i of the row; position -1: there is none
       const int32_t* const pages = P.table + r.b * P.table_stride;
       const int end = (r.tile0 + r.tiles) * per_tile;
       auto look_up = [&](int piece, int& pos, int& page) {
@@ -163,34 +182,32 @@ decode_sm100_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         if (__any_sync(0xffffffffu, bad) && lane == 0) ctl->bad = 1 + r.b;
         const int n_keys = pos < 0 || bad ? 0 : min(P.unit, r.len - pos), n_hidden = bad ? min(P.unit, r.len - pos) : 0;
         const int slot = pos < 0 ? 0 : pos % P.page;
-        for (int g = 0; g < 32 && first + g < end; g += per_tile) {
-          if (used >= STAGES) ok = warp_wait(b_free + 8 * stage, par, abort_flag, budget);
+        const uint32_t there = __ballot_sync(0xffffffffu, n_keys > 0);
+        for (int g = 0; g < 32 && first + g < end; g += per_stage) {
+          if (used >= STAGES) ok = quick_wait(b_free + 8 * stage, par, abort_flag, budget);
           if (!ok) break;
-          const bool mine = lane >= g && lane < g + per_tile;
-          const uint32_t loads = __ballot_sync(0xffffffffu, mine && n_keys > 0);
-          // slabs: 16 keys each, unit / 16 per piece
-          if (mine) {
-            for (int s = 0; s < P.unit / 16; ++s) {
-              SlabInfo* to = &ctl->slab[stage][(lane - g) * (P.unit / 16) + s];
-              to->pos = pos + 16 * s;
-              to->n = max(0, min(16, n_keys - 16 * s));
-              to->hidden = max(0, min(16, n_hidden - 16 * s));
-            }
+          const uint32_t loads = there & (((1u << per_stage) - 1u) << g);      // the pieces behind `end` are not there
+          const bool mine = lane >= g && lane < g + per_stage;
+          const uint32_t bar = b_full + 8 * stage;
+          if (first_warp && mine) {                  // units of 16 keys
+            for (int u = 0; u < P.unit / 16; ++u)
+              *reinterpret_cast<int4*>(&ctl->slab[stage][(lane - g) * (P.unit / 16) + u]) =
+                  make_int4(pos + 16 * u, max(0, min(16, n_keys - 16 * u)), max(0, min(16, n_hidden - 16 * u)), 0);
           }
           __syncwarp();
-          const uint32_t bar = b_full + 8 * stage;
           if (lane == 0) {
-            __threadfence_block();
-            if (loads != 0u) mbar_arrive_expect_tx(bar, (uint32_t)__popc(loads) * piece_bytes * 2u * PANELS);
+            if (loads != 0u) mbar_arrive_expect_tx(bar, (uint32_t)__popc(loads) * piece_panel * PANELS);
             else mbar_arrive(bar);
           }
           __syncwarp();
           if (mine && n_keys > 0) {
-            const uint32_t dst = ring + (uint32_t)stage * STAGE + (uint32_t)(lane - g) * piece_bytes;
+            const uint32_t dst = ring + (uint32_t)stage * STAGE + (first_warp ? 0u : HALF) + (uint32_t)(lane - g) * piece_panel * PANELS;
+            if (P.one_box) {
+              tma_load_5d(dst, map, bar, 0, slot, 0, r.hk, page);
+            } else {
 #pragma unroll
-            for (int pn = 0; pn < PANELS; ++pn) tma_load_4d(dst + pn * PANEL, &tm_k, bar, pn * 64, r.hk, slot, page);
-#pragma unroll
-            for (int pn = 0; pn < PANELS; ++pn) tma_load_4d(dst + HALF + pn * PANEL, &tm_v, bar, pn * 64, r.hk, slot, page);
+              for (int pn = 0; pn < PANELS; ++pn) tma_load_5d(dst + pn * piece_panel, map, bar, pn * 64, slot, 0, r.hk, page);
+            }
           }
           ++used;
           if (++stage == STAGES) {
@@ -203,41 +220,60 @@ decode_sm100_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         page = next_page;
       }
     }
-    {                                                // copies still in flight land before the CTA leaves (bounded)
-      for (int back = 1; back <= STAGES && used - back >= 0; ++back) {
-        const int c = used - back;
-        mbar_wait_clock(b_full + 8u * (uint32_t)(c % STAGES), (uint32_t)(c / STAGES) & 1u, budget >> 4);
-      }
+    // copies still in flight land before the CTA leaves (bounded)
+    for (int back = 1; back <= STAGES && used - back >= 0; ++back) {
+      const int c = used - back;
+      mbar_wait_clock(b_full + 8u * (uint32_t)(c % STAGES), (uint32_t)(c / STAGES) & 1u, budget >> 4);
     }
   } else {
     // =============================== products and softmax ===============================
     const int slab = warp & 3, half = warp >> 2, g = lane >> 2, t4 = lane & 3;
     const int head_base = wide ? half * 16 : 0;      // first of the warp's 16 heads in the chunk
+    const uint32_t o_panel = HALVES ? (uint32_t)half * (COLUMNS / 64) : 0u;      // first panel of the warp's columns of O
     bool ok = *abort_flag == 0;
-    int n_rows = 0, stage = 0, tile_count = 0;
+    int n_rows = 0, stage = 0, count = 0;
     uint32_t par = 0u, meet_par = 0u;
     const uint32_t b_meet = smem_u32(&ctl->meet);
-    // ldmatrix addresses: row of the slab and 16-byte column that this lane points at
-    const uint32_t k_row = (uint32_t)(slab * 16 + (lane & 7) + ((lane >> 4) << 3)), k_col = (uint32_t)((lane >> 3) & 1);
-    const uint32_t v_row = (uint32_t)(slab * 16 + (lane & 15)), v_col = (uint32_t)(lane >> 4);
+    // where this lane points at in K and V of a stage for ldmatrix, per unit of 16 keys: a piece holds its panels one behind the other
+    const uint32_t k_row = (uint32_t)((lane & 7) + ((lane >> 4) << 3)), k_col = (uint32_t)((lane >> 3) & 1);
+    const uint32_t v_row = (uint32_t)(lane & 15), v_col = (uint32_t)(lane >> 4);
+    uint32_t unit_at[UNITS];
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) {
+      const int key = (slab * UNITS + u) * 16;
+      unit_at[u] = (uint32_t)(key / P.unit) * piece_panel * PANELS + (uint32_t)(key % P.unit) * 128u;
+    }
+    const uint32_t q_smem = smem_u32(part) + (uint32_t)(lane & 15) * D * 2u;
     while (ok) {
-      ok = warp_wait(b_row_full + 8 * (n_rows & 1), (uint32_t)(n_rows >> 1) & 1u, abort_flag, budget);
+      ok = quick_wait(b_row_full + 8 * (n_rows & 1), (uint32_t)(n_rows >> 1) & 1u, abort_flag, budget);
       if (!ok) break;
       const DecodeRow r = ctl->row[n_rows & 1];
       if (r.b < 0) break;
       const int head0 = r.hk * P.group + r.chunk * P.chunk_heads, heads = min(P.chunk_heads, P.group - r.chunk * P.chunk_heads);
       // Q as left operands: heads g and g + 8 of the warp's 16
-      uint32_t q[KSTEPS][4];
-#pragma unroll
-      for (int ks = 0; ks < KSTEPS; ++ks)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int h = head_base + g + (e & 1) * 8, d = ks * 16 + t4 * 2 + (e >> 1) * 8;
-          q[ks][e] = h < heads && d < P.headdim ? *reinterpret_cast<const uint32_t*>(static_cast<const T*>(P.q) + r.b * P.q_s[0] + (head0 + h) * P.q_s[1] + d) : 0u;
+      uint32_t q[HALVES ? 1 : KSTEPS][4];
+      const T* const q_row = static_cast<const T*>(P.q) + r.b * P.q_s[0] + head0 * P.q_s[1];
+      if (HALVES) {                                  // [16][D] where the parts are exchanged later, 16-byte columns swapped by row
+        for (int i = tid; i < 16 * (D / 8); i += kConsumers * 32) {
+          const int h = i / (D / 8), c = i % (D / 8);
+          uint4 x = make_uint4(0u, 0u, 0u, 0u);
+          if (h < heads && c * 8 < P.headdim) x = *reinterpret_cast<const uint4*>(q_row + h * P.q_s[1] + c * 8);
+          *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(part) + h * (D * 2) + ((c ^ (h & 7)) << 4)) = x;
         }
-      float o[D / 8][4];
+        ok = meet(b_meet, meet_par, abort_flag, budget);
+        if (!ok) break;
+      } else {
 #pragma unroll
-      for (int i = 0; i < D / 8; ++i)
+        for (int ks = 0; ks < KSTEPS; ++ks)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int h = head_base + g + (e & 1) * 8, d = ks * 16 + t4 * 2 + (e >> 1) * 8;
+            q[HALVES ? 0 : ks][e] = h < heads && d < P.headdim ? *reinterpret_cast<const uint32_t*>(q_row + h * P.q_s[1] + d) : 0u;
+          }
+      }
+      float o[COLUMNS / 8][4];
+#pragma unroll
+      for (int i = 0; i < COLUMNS / 8; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
       float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
@@ -246,56 +282,81 @@ decode_sm100_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         if (head_base + g < heads) score0 = P.sp.scores + ((long long)r.b * P.nhead_q + head0 + head_base + g) * P.capacity;
         if (head_base + g + 8 < heads) score1 = P.sp.scores + ((long long)r.b * P.nhead_q + head0 + head_base + g + 8) * P.capacity;
       }
-      for (int i = 0; i < r.tiles; ++i, ++tile_count) {
-        const bool mine = wide || (tile_count & 1) == half;
+      // a stage holds the same number of pieces whatever the row's first tile is, so the last one of a row may be half empty, and
+      // of every 32 pieces that are looked up together the last stage is full
+      const int n_stages = (r.tiles * kDecodeTile + Shape<D>::kKeys - 1) / Shape<D>::kKeys;
+      for (int i = 0; i < n_stages; ++i, ++count) {
+        const bool mine = all || (count & 1) == half;
         if (mine) {
-          ok = warp_wait(b_full + 8 * stage, par, abort_flag, budget);
+          ok = quick_wait(b_full + 8 * stage, par, abort_flag, budget);
           if (!ok) break;
-          const volatile SlabInfo* info = &ctl->slab[stage][slab];
-          const int n = info->n, pos = info->pos, hidden = info->hidden;
-          if (n > 0) {
-            const uint32_t k_at = ring + (uint32_t)stage * STAGE, v_at = k_at + HALF;
-            float s[2][4];
+          int4 info[UNITS];
+          int least = 16, most = 0, hidden = 0;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[0][e] = s[1][e] = 0.f;
+          for (int u = 0; u < UNITS; ++u) {
+            info[u] = *reinterpret_cast<const int4*>(&ctl->slab[stage][slab * UNITS + u]);
+            least = min(least, info[u].y);
+            most = max(most, info[u].y);
+            hidden |= info[u].z;
+          }
+          if (most > 0) {
+            const uint32_t k_at = ring + (uint32_t)stage * STAGE, v_at = k_at + HALF;
+            float s[2 * UNITS][4];
+#pragma unroll
+            for (int j = 0; j < 2 * UNITS; ++j)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) s[j][e] = 0.f;
 #pragma unroll
             for (int ks = 0; ks < KSTEPS; ++ks) {
-              uint32_t f[4];
               const uint32_t col = (uint32_t)(ks & 3) * 2u + k_col;
-              ldmatrix4(k_at + (uint32_t)(ks >> 2) * PANEL + k_row * 128u + ((col ^ (k_row & 7u)) << 4), f);
-              mma16816<BF16>(s[0], q[ks], f[0], f[1]);
-              mma16816<BF16>(s[1], q[ks], f[2], f[3]);
+              if (HALVES) ldmatrix4(q_smem + (((uint32_t)(ks * 2) + (uint32_t)(lane >> 4)) ^ (uint32_t)(lane & 7)) * 16u, q[0]);
+#pragma unroll
+              for (int u = 0; u < UNITS; ++u) {
+                uint32_t f[4];
+                ldmatrix4(k_at + unit_at[u] + (uint32_t)(ks >> 2) * piece_panel + k_row * 128u + ((col ^ (k_row & 7u)) << 4), f);
+                mma16816<BF16>(s[2 * u], q[HALVES ? 0 : ks], f[0], f[1]);
+                mma16816<BF16>(s[2 * u + 1], q[HALVES ? 0 : ks], f[2], f[3]);
+              }
             }
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
+            for (int j = 0; j < 2 * UNITS; ++j)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                s[j][e] *= P.scale_log2;
-                if (j * 8 + t4 * 2 + (e & 1) >= n) s[j][e] = -INFINITY;
-              }
-            if (P.weights != nullptr) {
+              for (int e = 0; e < 4; ++e) s[j][e] *= P.scale_log2;
+            if (least < 16) {
 #pragma unroll
-              for (int j = 0; j < 2; ++j)
+              for (int j = 0; j < 2 * UNITS; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  if ((j & 1) * 8 + t4 * 2 + (e & 1) >= info[j >> 1].y) s[j][e] = -INFINITY;
+            }
+            if (P.weights != nullptr && !(HALVES && half)) {
+#pragma unroll
+              for (int j = 0; j < 2 * UNITS; ++j)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                  const int key = j * 8 + t4 * 2 + e;
-                  if (key < n) {
-                    if (score0 != nullptr) score0[pos + key] = s[j][e];
-                    if (score1 != nullptr) score1[pos + key] = s[j][2 + e];
+                  const int key = (j & 1) * 8 + t4 * 2 + e;
+                  if (key < info[j >> 1].y) {
+                    if (score0 != nullptr) score0[info[j >> 1].x + key] = s[j][e];
+                    if (score1 != nullptr) score1[info[j >> 1].x + key] = s[j][2 + e];
                   }
                 }
             }
-            float x0 = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1])), x1 = fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3]));
-            x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 1));
-            x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 1));
-            x0 = fmaxf(m0, fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 2)));
-            x1 = fmaxf(m1, fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 2)));
-            if (__any_sync(0xffffffffu, x0 > m0 || x1 > m1)) {
+            float x0 = m0, x1 = m1;
+#pragma unroll
+            for (int j = 0; j < 2 * UNITS; ++j) {
+              x0 = fmaxf(x0, fmaxf(s[j][0], s[j][1]));
+              x1 = fmaxf(x1, fmaxf(s[j][2], s[j][3]));
+            }
+            if (__any_sync(0xffffffffu, x0 > m0 || x1 > m1)) {       // some row's maximum grows: the quads agree on it, O and the sums follow
+              x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 1));
+              x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 1));
+              x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 2));
+              x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 2));
               const float a0 = x0 == -INFINITY ? 1.f : ex2_approx(m0 - x0), a1 = x1 == -INFINITY ? 1.f : ex2_approx(m1 - x1);
               l0 *= a0;
               l1 *= a1;
 #pragma unroll
-              for (int d = 0; d < D / 8; ++d) {
+              for (int d = 0; d < COLUMNS / 8; ++d) {
                 o[d][0] *= a0;
                 o[d][1] *= a0;
                 o[d][2] *= a1;
@@ -305,38 +366,44 @@ decode_sm100_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
               m1 = x1;
             }
             const float r0 = m0 == -INFINITY ? 0.f : m0, r1 = m1 == -INFINITY ? 0.f : m1;
-            uint32_t p[4];
+            uint32_t p[UNITS][4];
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
+            for (int j = 0; j < 2 * UNITS; ++j) {
               const float p0 = ex2_approx(s[j][0] - r0), p1 = ex2_approx(s[j][1] - r0), p2 = ex2_approx(s[j][2] - r1), p3 = ex2_approx(s[j][3] - r1);
               l0 += p0 + p1;
               l1 += p2 + p3;
-              p[2 * j] = pack2<BF16>(p0, p1);
-              p[2 * j + 1] = pack2<BF16>(p2, p3);
+              p[j >> 1][2 * (j & 1)] = pack2<BF16>(p0, p1);
+              p[j >> 1][2 * (j & 1) + 1] = pack2<BF16>(p2, p3);
             }
-            if (n < 16) {                            // rows of V behind the length: zeros
-              if (lane >= n && lane < 16)
+            if (least < 16) {                        // rows of V that take no part: zeros
 #pragma unroll
-                for (int pn = 0; pn < PANELS; ++pn)
+              for (int u = 0; u < UNITS; ++u)
+                if (lane >= info[u].y && lane < 16)
 #pragma unroll
-                  for (int c = 0; c < 8; ++c) st_shared_v4(v_at + pn * PANEL + (uint32_t)(slab * 16 + lane) * 128u + c * 16u, 0u, 0u, 0u, 0u);
+                  for (int pn = 0; pn < PANELS; ++pn)
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) st_shared_v4(v_at + unit_at[u] + pn * piece_panel + (uint32_t)lane * 128u + c * 16u, 0u, 0u, 0u, 0u);
               fence_proxy_async();
               __syncwarp();
             }
 #pragma unroll
-            for (int c = 0; c < D / 16; ++c) {
-              uint32_t f[4];
+            for (int c = 0; c < COLUMNS / 16; ++c) {
               const uint32_t col = (uint32_t)(c & 3) * 2u + v_col;
-              ldmatrix4_t(v_at + (uint32_t)(c >> 2) * PANEL + v_row * 128u + ((col ^ (v_row & 7u)) << 4), f);
-              mma16816<BF16>(o[2 * c], p, f[0], f[1]);
-              mma16816<BF16>(o[2 * c + 1], p, f[2], f[3]);
+#pragma unroll
+              for (int u = 0; u < UNITS; ++u) {
+                uint32_t f[4];
+                ldmatrix4_t(v_at + unit_at[u] + ((uint32_t)(c >> 2) + o_panel) * piece_panel + v_row * 128u + ((col ^ (v_row & 7u)) << 4), f);
+                mma16816<BF16>(o[2 * c], p[u], f[0], f[1]);
+                mma16816<BF16>(o[2 * c + 1], p[u], f[2], f[3]);
+              }
             }
           }
-          if (hidden > 0 && P.weights != nullptr) {   // keys on a page that does not exist: no weight
-            if (t4 == 0)
-              for (int key = 0; key < hidden; ++key) {
-                if (score0 != nullptr) score0[pos + key] = -INFINITY;
-                if (score1 != nullptr) score1[pos + key] = -INFINITY;
+          if (hidden != 0 && P.weights != nullptr && t4 == 0) {      // keys on a page that does not exist: no weight
+#pragma unroll
+            for (int u = 0; u < UNITS; ++u)
+              for (int key = 0; key < info[u].z; ++key) {
+                if (score0 != nullptr) score0[info[u].x + key] = -INFINITY;
+                if (score1 != nullptr) score1[info[u].x + key] = -INFINITY;
               }
           }
           __syncwarp();
@@ -358,58 +425,57 @@ decode_sm100_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         *reinterpret_cast<float2*>(ctl->ml[warp][g + 8]) = make_float2(m1, l1);
       }
       ok = meet(b_meet, meet_par, abort_flag, budget);
-      if (ok) {
-        const int w0 = wide ? half * 4 : 0, w1 = wide ? w0 + 4 : kConsumers;       // the warps that share this warp's heads
-        float t0 = -INFINITY, t1 = -INFINITY;
-        for (int w = w0; w < w1; ++w) {
-          t0 = fmaxf(t0, ctl->ml[w][g][0]);
-          t1 = fmaxf(t1, ctl->ml[w][g + 8][0]);
-        }
-        const float f0 = m0 == -INFINITY ? 0.f : ex2_approx(m0 - t0), f1 = m1 == -INFINITY ? 0.f : ex2_approx(m1 - t1);
-        const long long part_slot = 2ll * blockIdx.x + max(r.slot, 0);
+      if (!ok) break;
+      const int w0 = all ? half * 4 : 0, w1 = all ? w0 + 4 : kConsumers;         // the warps that share this warp's heads and columns
+      float t0 = -INFINITY, t1 = -INFINITY;
+      for (int w = w0; w < w1; ++w) {
+        t0 = fmaxf(t0, ctl->ml[w][g][0]);
+        t1 = fmaxf(t1, ctl->ml[w][g + 8][0]);
+      }
+      const float f0 = m0 == -INFINITY ? 0.f : ex2_approx(m0 - t0), f1 = m1 == -INFINITY ? 0.f : ex2_approx(m1 - t1);
+      const long long part_slot = 2ll * blockIdx.x + max(r.slot, 0);
 #pragma unroll
-        for (int c = 0; c < PANELS; ++c) {
+      for (int c = 0; c < COLUMNS / 64; ++c) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            float* to = part + (warp * 16 + g) * 64 + (i ^ g) * 8 + t4 * 2;      // groups of 8 columns swapped by row: no bank conflicts
-            *reinterpret_cast<float2*>(to) = make_float2(o[c * 8 + i][0] * f0, o[c * 8 + i][1] * f0);
-            *reinterpret_cast<float2*>(to + 8 * 64) = make_float2(o[c * 8 + i][2] * f1, o[c * 8 + i][3] * f1);
-          }
-          if (!(ok = meet(b_meet, meet_par, abort_flag, budget))) break;
-          // thread = (head, 4 columns); 32 heads in two goes
-          for (int hh = 0; hh < (wide ? 2 : 1); ++hh) {
-            const int hl = tid >> 4, col = (tid & 15) * 4, head = hh * 16 + hl;
-            const int a = wide ? hh * 4 : 0, b = wide ? a + 4 : kConsumers;
-            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-            float mt = -INFINITY, lt = 0.f;
-            for (int w = a; w < b; ++w) mt = fmaxf(mt, ctl->ml[w][hl][0]);
-            for (int w = a; w < b; ++w) {
-              const float4 y = *reinterpret_cast<const float4*>(part + (w * 16 + hl) * 64 + (((col >> 3) ^ (hl & 7)) << 3) + (col & 7));
-              x.x += y.x;
-              x.y += y.y;
-              x.z += y.z;
-              x.w += y.w;
-              const float mw = ctl->ml[w][hl][0];
-              lt += mw == -INFINITY ? ctl->ml[w][hl][1] : ctl->ml[w][hl][1] * ex2_approx(mw - mt);
-            }
-            if (head < heads) {
-              if (r.slot >= 0) {
-                *reinterpret_cast<float4*>(P.sp.part_o + (part_slot * kDecodeHeads + head) * D + c * 64 + col) = x;
-                if (c == 0 && col == 0) *reinterpret_cast<float2*>(P.sp.part_ml + (part_slot * kDecodeHeads + head) * 2) = make_float2(mt, lt);
-              } else {
-                const bool none = mt == -INFINITY && lt == 0.f;
-                const float inv = none ? 0.f : 1.f / lt;
-                const int d = c * 64 + col;
-                if (d < P.headdim)
-                  *reinterpret_cast<uint2*>(static_cast<T*>(P.o) + r.b * P.o_s[0] + (head0 + head) * P.o_s[1] + d) =
-                      none ? make_uint2(0u, 0u) : make_uint2(pack2<BF16>(x.x * inv, x.y * inv), pack2<BF16>(x.z * inv, x.w * inv));
-                if (c == 0 && col == 0 && P.lse != nullptr)
-                  P.lse[(long long)r.b * P.nhead_q + head0 + head] = none ? -INFINITY : (mt + log2f(lt)) * kDecodeLn2;
-              }
-            }
-          }
-          if (!(ok = meet(b_meet, meet_par, abort_flag, budget))) break;           // before the next columns, or the next row's statistics
+        for (int i = 0; i < 8; ++i) {
+          float* to = part + (warp * 16 + g) * 64 + (i ^ g) * 8 + t4 * 2;        // groups of 8 columns swapped by row: no bank conflicts
+          *reinterpret_cast<float2*>(to) = make_float2(o[c * 8 + i][0] * f0, o[c * 8 + i][1] * f0);
+          *reinterpret_cast<float2*>(to + 8 * 64) = make_float2(o[c * 8 + i][2] * f1, o[c * 8 + i][3] * f1);
         }
+        if (!(ok = meet(b_meet, meet_par, abort_flag, budget))) break;
+        // thread = (head, 4 columns); 32 heads, or both halves of the columns, in two goes
+        for (int hh = 0; hh < (all ? 2 : 1); ++hh) {
+          const int hl = tid >> 4, col = (tid & 15) * 4, head = HALVES ? hl : hh * 16 + hl;
+          const int a = all ? hh * 4 : 0, b = all ? a + 4 : kConsumers;
+          const int d = (HALVES ? hh * COLUMNS : 0) + c * 64 + col;
+          float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+          float mt = -INFINITY, lt = 0.f;
+          for (int w = a; w < b; ++w) mt = fmaxf(mt, ctl->ml[w][hl][0]);
+          for (int w = a; w < b; ++w) {
+            const float4 y = *reinterpret_cast<const float4*>(part + (w * 16 + hl) * 64 + (((col >> 3) ^ (hl & 7)) << 3) + (col & 7));
+            x.x += y.x;
+            x.y += y.y;
+            x.z += y.z;
+            x.w += y.w;
+            const float mw = ctl->ml[w][hl][0];
+            lt += mw == -INFINITY ? ctl->ml[w][hl][1] : ctl->ml[w][hl][1] * ex2_approx(mw - mt);
+          }
+          if (head < heads) {
+            if (r.slot >= 0) {
+              *reinterpret_cast<float4*>(P.sp.part_o + (part_slot * kDecodeHeads + head) * D + d) = x;
+              if (d == 0) *reinterpret_cast<float2*>(P.sp.part_ml + (part_slot * kDecodeHeads + head) * 2) = make_float2(mt, lt);
+            } else {
+              const bool none = mt == -INFINITY && lt == 0.f;
+              const float inv = none ? 0.f : 1.f / lt;
+              if (d < P.headdim)
+                *reinterpret_cast<uint2*>(static_cast<T*>(P.o) + r.b * P.o_s[0] + (head0 + head) * P.o_s[1] + d) =
+                    none ? make_uint2(0u, 0u) : make_uint2(pack2<BF16>(x.x * inv, x.y * inv), pack2<BF16>(x.z * inv, x.w * inv));
+              if (d == 0 && P.lse != nullptr)
+                P.lse[(long long)r.b * P.nhead_q + head0 + head] = none ? -INFINITY : (mt + log2f(lt)) * kDecodeLn2;
+            }
+          }
+        }
+        if (!(ok = meet(b_meet, meet_par, abort_flag, budget))) break;           // before the next columns, or the next row's statistics
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(b_row_done + 8 * (n_rows & 1));
@@ -427,13 +493,19 @@ decode_sm100_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
   }
 }
 
-// 4-D map over pages of a cache: dims (headdim, heads, slots, pages), box (64, 1, unit, 1).
+// 5-D map over the pages of a cache: dims (columns, slots, panels, heads, pages), box (64, unit, panels, 1, 1).  Head dimensions that are no
+// multiple of 64 are one panel of headdim columns, so that the hardware fills the columns behind them with zeros.
+// The L2 fetches no more than what lies together of a kv-head: with 64 columns and heads inside the slots (128 bytes a row), fetches of
+// 256 bytes brought the next head along (16 x 24576 keys, 8 heads: 198 us, 128 bytes as below: 160 us).
 bool encode_cache_map(EncodeTiledFn fn, CUtensorMap* map, bool bf16, const void* base, const DecodeParams& P, const long long* s) {
-  cuuint64_t dims[4] = {(cuuint64_t)P.headdim, (cuuint64_t)P.nhead_k, (cuuint64_t)P.page, (cuuint64_t)P.num_pages};
-  cuuint64_t strides[3] = {(cuuint64_t)s[2] * 2ull, (cuuint64_t)s[1] * 2ull, (cuuint64_t)s[0] * 2ull};
-  cuuint32_t box[4] = {64u, 1u, (cuuint32_t)P.unit, 1u}, estr[4] = {1u, 1u, 1u, 1u};
-  return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), dims, strides, box, estr,
-            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  const int panels = P.one_box ? P.headdim / 64 : 1;
+  cuuint64_t dims[5] = {(cuuint64_t)(P.one_box ? 64 : P.headdim), (cuuint64_t)P.page, (cuuint64_t)panels, (cuuint64_t)P.nhead_k, (cuuint64_t)P.num_pages};
+  cuuint64_t strides[4] = {(cuuint64_t)s[1] * 2ull, 128ull, (cuuint64_t)s[2] * 2ull, (cuuint64_t)s[0] * 2ull};
+  const long long run = (s[1] == P.headdim ? 2ll * P.page : 2ll) * P.headdim;
+  const CUtensorMapL2promotion promotion = run >= 256 ? CU_TENSOR_MAP_L2_PROMOTION_L2_256B : run >= 128 ? CU_TENSOR_MAP_L2_PROMOTION_L2_128B : CU_TENSOR_MAP_L2_PROMOTION_L2_64B;
+  cuuint32_t box[5] = {64u, (cuuint32_t)P.unit, P.one_box ? (cuuint32_t)(P.d_pad / 64) : 1u, 1u, 1u}, estr[5] = {1u, 1u, 1u, 1u, 1u};
+  return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5, const_cast<void*>(base), dims, strides, box, estr,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, promotion, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <int D, bool BF16>

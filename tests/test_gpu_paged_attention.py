@@ -119,6 +119,18 @@ def test_long_rows_are_split_and_joined(dtype, hq, hk, d, lens):
         assert torch.equal(out, hb.paged_attention(q, c["k"], c["v"], c["table"], c["cache_lens"]))
 
 
+@pytest.mark.parametrize("dtype,hq,hk,d,page", [(torch.bfloat16, 16, 4, 64, 64), (torch.float16, 8, 4, 128, 16), (torch.bfloat16, 16, 4, 256, 64), (torch.bfloat16, 36, 2, 128, 32),
+                                               (torch.float16, 40, 2, 256, 16)])
+def test_many_rounds_of_the_ring(dtype, hq, hk, d, page):
+    """Every CTA goes through its stages dozens of times, over several rows."""
+    import hbsattn_b200 as hb
+    lens = [20000, 15001, 9000, 20011, 64, 17000, 12345, 19999]
+    c = make_cache(70, lens, hk, d, page, dtype, fill=0.0)
+    q = _q(71, len(lens), hq, d, dtype)
+    out, lse = hb.paged_attention(q, c["k"], c["v"], c["table"], c["cache_lens"], return_lse=True)
+    _check(q, c, out, lse)
+
+
 @pytest.mark.parametrize("batch,n,hq,hk,d", [(300, 40, 8, 2, 64), (1500, 5, 1, 1, 32), (64, 700, 16, 8, 128)])
 def test_many_sequences(batch, n, hq, hk, d):
     import hbsattn_b200 as hb
