@@ -22,15 +22,31 @@ template <> __device__ __forceinline__ float to_f<float>(float x) { return x; }
 template <> __device__ __forceinline__ float to_f<__half>(__half x) { return __half2float(x); }
 template <> __device__ __forceinline__ float to_f<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
 
-// -lse log2 e of every row (-inf: nothing to add), the cleared work cursor, zeros for keys outside every sample.
+// -lse log2 e of every row in the order of the tiles (-inf: nothing to add), zeros for keys outside every sample, the cleared work cursor.
 __global__ void __launch_bounds__(256) key_weights_prep_kernel(const __grid_constant__ KeyWeightsParams P, const float* __restrict__ lse) {
-  const bool all = P.ws.status[0] != HBSA_STATUS_OK;
+  const Problem& p = P.p;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (blockIdx.x == 0 && threadIdx.x < 32) P.sp.cursor[threadIdx.x] = 0;
-  key_weights_outside(P, all);
-  const long long n = (long long)P.total_q * P.p.nhead_q;
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += gridDim.x * 256ll) {
-    const float l = lse[i];
-    P.sp.neg_lse[i] = l == -INFINITY ? -INFINITY : -l * kLog2e;
+  asm volatile("griddepcontrol.wait;" ::: "memory");               // the schedule
+  const bool ok = P.ws.status[0] == HBSA_STATUS_OK;
+  key_weights_outside(P, !ok);
+  if (!ok) return;
+  // a warp takes 256 values of a q-block at a time, in the order of lse (rows, then heads)
+  const int lane = threadIdx.x & 31, n = p.qbs * p.nhead_q, chunks = (n + 255) / 256;
+  const long long todo = (long long)p.num_q_block * chunks;
+  for (long long u = blockIdx.x * 8 + (threadIdx.x >> 5); u < todo; u += gridDim.x * 8) {
+    const int qb = (int)(u / chunks), first = (int)(u % chunks) * 256 + lane;
+    const RowGeom g = row_geometry(p, P.ws.cnq, P.ws.cnk, P.ws.qb2b, qb);
+    const float* src = lse + (long long)g.q_begin * p.nhead_q;
+    const int there = (g.q_end - g.q_begin) * p.nhead_q;
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = first + 32 * e < there ? src[first + 32 * e] : -INFINITY;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int i = first + 32 * e, tok = i / p.nhead_q, h = i - tok * p.nhead_q;
+      if (i < n) P.sp.neg_lse[(((long long)(h >> P.gp_shift) * p.num_q_block + qb) * p.qbs + tok) * P.gp + (h & (P.gp - 1))] = x[e] == -INFINITY ? -INFINITY : -x[e] * kLog2e;
+    }
   }
 }
 
@@ -79,7 +95,8 @@ __global__ void __launch_bounds__(kThreads) key_weights_generic_kernel(const __g
       }
       if (tid < kRows) {
         const int r = r0 + tid;
-        s_nl[tid] = r < n_rows ? P.sp.neg_lse[(long long)(q_begin + i * p.qbs + r / p.group) * p.nhead_q + hk * p.group + r % p.group] : -INFINITY;
+        const int h = hk * p.group + r % p.group;
+        s_nl[tid] = r < n_rows ? P.sp.neg_lse[(((long long)(h >> P.gp_shift) * p.num_q_block + qb0 + i) * p.qbs + r / p.group) * P.gp + (h & (P.gp - 1))] : -INFINITY;
       }
       __syncthreads();
       float tile_sum = 0.f;
@@ -131,7 +148,7 @@ size_t carve_key_weights(const hbsa_forward_args& a, char* base, KeyWeightsSpace
   char* p = base;
   auto take = [&](size_t bytes) { char* r = p; p += (bytes + 255) / 256 * 256; return r; };
   s->cursor = reinterpret_cast<unsigned long long*>(take(256));
-  s->neg_lse = reinterpret_cast<float*>(take((size_t)a.total_q * a.nhead_q * 4));
+  s->neg_lse = reinterpret_cast<float*>(take((size_t)a.num_q_block * a.q_block_size * a.nhead_q * 4));
   return (size_t)(p - base);
 }
 
@@ -142,7 +159,7 @@ size_t carve_key_weights(const hbsa_forward_args& a, char* base, KeyWeightsSpace
 extern "C" {
 
 size_t hbsa_key_weights_workspace_bytes(const hbsa_key_weights_args* args) {
-  if (!args || args->struct_bytes != sizeof(*args) || args->fwd.total_q < 0 || args->fwd.nhead_q <= 0) return 0;
+  if (!args || args->struct_bytes != sizeof(*args) || args->fwd.num_q_block <= 0 || args->fwd.q_block_size <= 0 || args->fwd.nhead_q <= 0) return 0;
   hbsa::KeyWeightsSpace s;
   return hbsa::carve_key_weights(args->fwd, nullptr, &s);
 }
@@ -179,9 +196,23 @@ int hbsa_key_weights(const hbsa_key_weights_args* args, void* stream_) {
   auto failed = [](cudaError_t e) { return set_last_error("hbsa_key_weights: %s", cudaGetErrorString(e)), (int)e; };
   cudaError_t e = launch_schedule(P.p, P.ws, nullptr, stream);
   if (e != cudaSuccess) return failed(e);
-  const long long rows = ((long long)a.total_q * a.nhead_q + 255) / 256, most = 8ll * sm100_sm_count();
-  key_weights_prep_kernel<<<(unsigned)(rows < 1 ? 1 : rows < most ? rows : most), 256, 0, stream>>>(P, a.lse);
-  if ((e = cudaGetLastError()) != cudaSuccess) return failed(e);
+  P.gp = 1;                                    // q-heads side by side in a tile: the largest power of two that divides the group
+  P.gp_shift = 0;
+  while (P.gp < 64 && P.p.group % (P.gp * 2) == 0) {
+    P.gp *= 2;
+    ++P.gp_shift;
+  }
+  const long long warps = ((long long)a.num_q_block * (((long long)a.q_block_size * a.nhead_q + 255) / 256) + 7) / 8, most = 8ll * sm100_sm_count();
+  cudaLaunchAttribute attr[1] = {};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(warps < most ? warps : most));
+  cfg.blockDim = dim3(256);
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if ((e = cudaLaunchKernelEx(&cfg, key_weights_prep_kernel, P, static_cast<const float*>(a.lse))) != cudaSuccess) return failed(e);
   if (impl == HBSA_IMPL_SM100) {
     const char* text = "";
     rc = launch_key_weights_sm100(P, a, stream, &text);

@@ -6,7 +6,8 @@ namespace hbsa {
 
 struct KeyWeightsSpace {
   unsigned long long* cursor;  // [32] word 0: next item, word 1: CTAs that have left
-  float* neg_lse;              // [total_q, nhead_q] -lse log2 e; -inf: the row adds nothing
+  float* neg_lse;              // -lse log2 e; -inf: the row adds nothing.  [nhead_q / gp][num_q_block][q_block_size][gp], blocks filled up with
+                               // -inf: rows in the order of the tiles, every q-block on a 64-byte boundary whatever the samples' lengths
 };
 
 struct KeyWeightsParams {
@@ -17,8 +18,9 @@ struct KeyWeightsParams {
   int total_q, total_k;
   float scale_log2;
   // tensor-core kernel
-  int gp, gp_shift, n_head_sub, tt, nt;      // q-heads of a tile, tiles of heads per group, tokens and rows of a tile
-  int m_rows, n_msub;                        // keys of a stationary tile, tiles per k-block
+  int gp, gp_shift, n_head_sub, piece, piece_shift;      // q-heads of a piece, pieces of heads per group, rows of a piece
+  int one_box;                               // one copy brings all columns of a tile
+  int m_rows, n_msub, n_cols;                // keys of an item, items per k-block, columns of S
   long long total_items;
   long long wait_budget;
   int debug_stall;
