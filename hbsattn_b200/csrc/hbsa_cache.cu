@@ -1,7 +1,5 @@
 // Writing into a paged key-value cache, choosing what stays when it is cut down, and moving that together.
 // All three are bound by memory: every byte is read once and written once.
-#include <string.h>
-
 #include "sm100_common.cuh"
 
 namespace hbsa {
@@ -21,7 +19,8 @@ struct AppendParams {
   const int32_t *table, *lens, *cu;
   long long table_stride;
   int32_t *new_lens, *status;
-  int num_pages, page, capacity, batch, heads, units, total;
+  FastDiv page;
+  int num_pages, capacity, batch, heads, units, total;
   int flat;                              // the heads of a token follow one another: one run of heads * units
 };
 
@@ -39,7 +38,7 @@ __device__ __forceinline__ void append_status(const AppendParams& P) {
     const int end = (int)min((long long)len + n, (long long)P.capacity);
     bool bad = raw != len || (long long)len + n > P.capacity;
     if (end > len)
-      for (int i = len / P.page + tid % per; i <= (end - 1) / P.page; i += per) {
+      for (int i = P.page.quotient(len) + tid % per; i <= P.page.quotient(end - 1); i += per) {
         const int page = P.table[b * P.table_stride + i];
         bad |= page < 0 || page >= P.num_pages;
       }
@@ -65,7 +64,8 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ App
     const int b = sample_of_block(P.cu, P.batch, (int)tok);
     const long long pos = (long long)cut(P.lens[b], P.capacity) + (tok - P.cu[b]);
     if (pos >= P.capacity) continue;
-    const int page = P.table[b * P.table_stride + (int)pos / P.page], slot = (int)pos % P.page;
+    int slot;
+    const int page = P.table[b * P.table_stride + P.page.split((int)pos, slot)];
     if (page < 0 || page >= P.num_pages) continue;
     const U *ks = k + tok * P.k_s[0], *vs = v + tok * P.v_s[0];
     U *kd = kc + page * P.kc.s[0] + slot * P.kc.s[1], *vd = vc + page * P.vc.s[0] + slot * P.vc.s[1];
@@ -97,123 +97,276 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ App
 }
 
 // ------------------------------------------------------------------------------------------------------------------
-// Select: radix select of the smallest weight that stays, then one pass that writes positions in order.
-constexpr int kSelectThreads = 1024;
+// Select: radix select of the smallest weight that stays, then one pass that writes positions in order.  The digits are 11 bits of the distance
+// from the smallest weight above zero (or, where all of those stay, from the smallest of the rest): that keeps keys that nobody has looked at
+// out of the counts, where they would meet in one bin, and spreads weights of one size over many.  A cluster of 1 to 8 CTAs per row; counts
+// are exchanged through distributed shared memory.  Every warp has its run of positions, in registers where they fit, as numbers that tell by
+// themselves whether the position competes; where they do not fit, they are read again for every pass.  Bound by the instructions of its
+// passes (23.7 us for 128 rows of 16384 to 32768, 35 us while every pass compared positions): memory is busy for the first one only.
+constexpr int kSelectBins = 2048;
+constexpr uint32_t kGoes = 0u, kStays = 0xffffffffu, kZero = 0x80000000u;
 
-// Weights as unsigned numbers in the same order; both zeros are one, NaN is the largest.
+// Weights as unsigned numbers in the same order, from 0x007fffff to 0xff800000; both zeros are one (0x80000000), NaN is the next above them all.
 __device__ __forceinline__ uint32_t order_of(float x) {
-  if (x != x) return 0xffffffffu;
+  if (x != x) return 0xff800001u;
   const uint32_t u = __float_as_uint(x + 0.f);
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-__global__ void __launch_bounds__(kSelectThreads) select_keys_kernel(const __grid_constant__ hbsa_select_keys_args a) {
-  constexpr int WARPS = kSelectThreads / 32;
-  __shared__ int s_hist[256];
-  __shared__ int s_more[WARPS], s_ties[WARPS];
-  __shared__ uint32_t s_prefix;
+__device__ __forceinline__ int ld_cluster(uint32_t addr) {
+  int x;
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(x) : "r"(addr) : "memory");
+  return x;
+}
+
+// PER: positions of a lane that registers hold, 0: none.
+template <int PER, int THREADS>
+__global__ void __launch_bounds__(THREADS) select_keys_kernel(const __grid_constant__ hbsa_select_keys_args a, int ctas) {
+  constexpr int WARPS = THREADS / 32, BINS = kSelectBins / THREADS, STEP = PER > 0 ? PER : 8;      // bins of a thread, positions of a lane and go
+  __shared__ int s_hist[kSelectBins];
+  __shared__ int s_more[WARPS], s_ties[WARPS], s_sum[2];
+  __shared__ uint32_t s_range[4], s_prefix;
   __shared__ int s_need;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int b = blockIdx.x / a.nhead_k, h = blockIdx.x % a.nhead_k;
+  const int row = blockIdx.x / ctas, rank = blockIdx.x - row * ctas, b = row / a.nhead_k, h = row - b * a.nhead_k;
   const int len = cut(a.lens[b], a.max_len);
   const float* w = a.key_weights + b * a.weights_stride[0] + h * a.weights_stride[1];
-  int32_t* kept = a.kept + (long long)blockIdx.x * a.budget;
-  if (h == 0 && tid == 0) a.kept_lens[b] = min(len, a.budget);
-  if (len <= a.budget) {
-    for (int i = tid; i < a.budget; i += kSelectThreads) kept[i] = i < len ? i : -1;
+  int32_t* kept = a.kept + (long long)row * a.budget;
+  if (h == 0 && rank == 0 && tid == 0) a.kept_lens[b] = min(len, a.budget);
+  if (len <= a.budget) {                                 // all CTAs of the cluster
+    for (int i = rank * THREADS + tid; i < a.budget; i += ctas * THREADS) kept[i] = i < len ? i : -1;
     return;
   }
   const int lo = a.n_sink, hi = len - a.n_recent;        // the positions that compete; n_sink + n_recent <= budget < len
   int need = a.budget - a.n_sink - a.n_recent;
-  uint32_t prefix = 0;
-  if (need > 0) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      if (tid < 256) s_hist[tid] = 0;
-      __syncthreads();
-      const uint32_t known = shift == 24 ? 0u : 0xffffffffu << (shift + 8);
-      for (int i = lo + tid; i < hi; i += kSelectThreads) {
-        const uint32_t u = order_of(w[i]);
-        if ((u & known) == prefix) atomicAdd(&s_hist[(u >> shift) & 255u], 1);
-      }
-      __syncthreads();
-      if (warp == 0) {                                   // the digit of the need-th largest: lane l holds digits 255 - 8 l ...
-        int c[8], sum = 0;
+  const int run = ((len + ctas - 1) / ctas + 31) & ~31, p0 = min(rank * run, len), p1 = min(p0 + run, len);      // this CTA's
+  const int seg = ((p1 - p0 + WARPS - 1) / WARPS + 31) & ~31, s0 = min(p0 + warp * seg, p1), s1 = min(s0 + seg, p1);     // this warp's
+  auto meet = [&]() {
+    if (ctas > 1) ptx::cluster_sync();
+    else __syncthreads();
+  };
+  // A number per position: its weight's while it competes; kStays for the first and last ones; kGoes behind the warp's.  Once the range that
+  // holds the answer is known, the distance from its low end, plus one, with kGoes below it and kStays above.
+  uint32_t u[STEP], low = 0u, high = 0u;
+  bool ranged = false;
+  auto place = [&](uint32_t x) { return x < low ? kGoes : x > high ? kStays : x - low + 1u; };
+  auto read = [&](int from) {
+#pragma unroll
+    for (int part = 0; part < STEP; part += 8) {
+      const int at = from + 32 * part;
+      if (at >= lo && at + 256 <= min(hi, s1)) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) u[part + e] = __float_as_uint(w[at + 32 * e + lane]);        // loads first
+#pragma unroll
+        for (int e = 0; e < 8; ++e) u[part + e] = order_of(__uint_as_float(u[part + e]));
+      } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          c[e] = s_hist[255 - 8 * lane - e];
-          sum += c[e];
+          const int i = at + 32 * e + lane;
+          u[part + e] = i >= s1 ? kGoes : i < lo || i >= hi ? kStays : order_of(w[i]);
         }
-        int incl = sum;
+      }
+      if (PER == 0 && ranged) {
 #pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-          const int y = __shfl_up_sync(0xffffffffu, incl, d);
-          if (lane >= d) incl += y;
+        for (int e = 0; e < 8; ++e) u[part + e] = place(u[part + e]);
+      }
+    }
+  };
+  // f(number, position of lane 0) for every 32 positions
+  auto each = [&](auto&& f) {
+    for (int at = s0; at < s1; at += 32 * STEP) {
+      if (PER == 0) read(at);
+#pragma unroll
+      for (int part = 0; part < STEP; part += 8)
+        if (at + 32 * part < s1) {
+#pragma unroll
+          for (int e = part; e < part + 8; ++e) f(u[e], at + 32 * e);
         }
-        int before = incl - sum;
-        if (before < need && incl >= need) {
+    }
+  };
+  if (tid < 4) s_range[tid] = tid < 2 ? 0xffffffffu : 0u;
+  if (PER > 0) read(s0);
+  uint32_t least = kStays;                               // the smallest number that stays
+  int ties = 0x7fffffff;                                 // and how many of it do
+  if (need > 0) {
+    // smallest of all (kGoes wraps around), smallest above zero (what is not above wraps), largest (kStays wraps), how many above zero
+    uint32_t least_all = 0xffffffffu, least_above = 0xffffffffu, most = 0u;
+    int above = 0;
+    each([&](uint32_t x, int) {
+      least_all = min(least_all, x - 1u);
+      least_above = min(least_above, x - (kZero + 1u));
+      most = max(most, x + 1u);
+      above += x > kZero;
+    });
+    least_all = __reduce_min_sync(0xffffffffu, least_all);
+    least_above = __reduce_min_sync(0xffffffffu, least_above);
+    most = __reduce_max_sync(0xffffffffu, most);
+    above = __reduce_add_sync(0xffffffffu, above);
+    __syncthreads();
+    if (lane == 0) {
+      atomicMin(&s_range[0], least_all);
+      atomicMin(&s_range[1], least_above);
+      atomicMax(&s_range[2], most);
+      atomicAdd(&s_range[3], (uint32_t)above);
+    }
+    meet();
+    least_all = least_above = 0xffffffffu;
+    most = 0u;
+    above = -a.n_sink - a.n_recent;                      // kStays were counted
+    for (int r = 0; r < ctas; ++r) {
+      const uint32_t at = ptx::map_to_rank(ptx::smem_u32(s_range), (uint32_t)r);
+      least_all = min(least_all, (uint32_t)ld_cluster(at));
+      least_above = min(least_above, (uint32_t)ld_cluster(at + 4u));
+      most = max(most, (uint32_t)ld_cluster(at + 8u));
+      above += ld_cluster(at + 12u);
+    }
+    if (need <= above) {
+      low = least_above + (kZero + 1u);
+      high = most - 1u;
+    } else {
+      need -= above;
+      low = least_all + 1u;
+      high = kZero;
+    }
+    ranged = true;
+    if (PER > 0) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            if (before < need && before + c[e] >= need) {
-              s_prefix = prefix | (uint32_t)(255 - 8 * lane - e) << shift;
-              s_need = need - before;
-              break;
-            }
-            before += c[e];
+      for (int e = 0; e < STEP; ++e) u[e] = place(u[e]);
+    }
+    int left = 32 - __clz((int)(high - low + 1u));       // low bits that are not settled: at most 31
+    uint32_t prefix = 0u;
+    while (left > 0) {
+      const int bits = min(left, 11), shift = left - bits;
+      const uint32_t bins = (1u << bits) - 1u, from = max(prefix, 1u), size = prefix + (1u << left) - from;
+      left = shift;
+      for (int i = tid; i < kSelectBins; i += THREADS) s_hist[i] = 0;
+      __syncthreads();
+      each([&](uint32_t x, int) {
+        if (x - from < size) atomicAdd(&s_hist[(x >> shift) & bins], 1);
+      });
+      meet();
+      // the digit of the need-th largest: thread t holds digits bins - BINS t downwards, over all CTAs
+      const int top = (int)bins - BINS * tid;
+      int c[BINS], sum = 0;
+#pragma unroll
+      for (int e = 0; e < BINS; ++e) c[e] = 0;
+      if (top >= 0) {
+        if (ctas == 1) {
+#pragma unroll
+          for (int e = 0; e < BINS; ++e) c[e] = top >= e ? s_hist[top - e] : 0;
+        } else {
+          for (int r = 0; r < ctas; ++r) {
+            const uint32_t at = ptx::map_to_rank(ptx::smem_u32(s_hist), (uint32_t)r);
+#pragma unroll
+            for (int e = 0; e < BINS; ++e) c[e] += top >= e ? ld_cluster(at + 4u * (uint32_t)(top - e)) : 0;
           }
         }
       }
+#pragma unroll
+      for (int e = 0; e < BINS; ++e) sum += c[e];
+      int incl = sum;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, incl, d);
+        if (lane >= d) incl += y;
+      }
+      if (lane == 31) s_more[warp] = incl;
       __syncthreads();
+      const int others = __reduce_add_sync(0xffffffffu, lane < warp ? s_more[lane < WARPS ? lane : 0] : 0);      // warps before this one
+      int before = others + incl - sum;
+      if (before < need && before + sum >= need) {       // one thread
+#pragma unroll
+        for (int e = 0; e < BINS; ++e) {
+          if (before < need && before + c[e] >= need) {
+            s_prefix = prefix | (uint32_t)(top - e) << shift;
+            s_need = need - before;
+            break;
+          }
+          before += c[e];
+        }
+      }
+      meet();                                            // also: all have read the counts
       prefix = s_prefix;
       need = s_need;
-      __syncthreads();
     }
+    least = prefix;
+    ties = need;
   }
-  // every weight above `prefix` stays, and the first `need` of those equal to it (none competes where nothing is needed)
-  const bool any = a.budget > a.n_sink + a.n_recent;
-  const int seg = (len + WARPS - 1) / WARPS, s0 = min(warp * seg, len), s1 = min(s0 + seg, len);
-  auto kind = [&](int i) -> int {                        // 2: stays, 1: a tie, 0: goes
-    if (i >= s1) return 0;
-    if (i < lo || i >= hi) return 2;
-    if (!any) return 0;
-    const uint32_t u = order_of(w[i]);
-    return u > prefix ? 2 : u == prefix ? 1 : 0;
-  };
-  int more = 0, ties = 0;
-  for (int i = s0 + lane; i < s1; i += 32) {
-    const int x = kind(i);
-    more += x == 2;
-    ties += x == 1;
-  }
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) {
-    more += __shfl_xor_sync(0xffffffffu, more, d);
-    ties += __shfl_xor_sync(0xffffffffu, ties, d);
-  }
+  // every number above `least` stays, and the first `ties` of those equal to it
+  int more = 0, equal = 0;
+  each([&](uint32_t x, int) {
+    more += x > least;
+    equal += x == least;
+  });
+  more = __reduce_add_sync(0xffffffffu, more);
+  equal = __reduce_add_sync(0xffffffffu, equal);
+  __syncthreads();
   if (lane == 0) {
     s_more[warp] = more;
-    s_ties[warp] = ties;
+    s_ties[warp] = equal;
   }
   __syncthreads();
+  // ties and positions that stay before this warp's: those of the CTAs before, then those of the warps before
   int out = 0, tie = 0;
-  for (int i = 0; i < warp; ++i) {
-    out += s_more[i] + min(max(need - tie, 0), s_ties[i]);
-    tie += s_ties[i];
+  if (ctas > 1) {
+    const int m = __reduce_add_sync(0xffffffffu, lane < WARPS ? s_more[lane] : 0), t = __reduce_add_sync(0xffffffffu, lane < WARPS ? s_ties[lane] : 0);
+    if (tid == 0) {
+      s_sum[0] = m;
+      s_sum[1] = t;
+    }
+    ptx::cluster_sync();
+    for (int r = 0; r < rank; ++r) {
+      const uint32_t at = ptx::map_to_rank(ptx::smem_u32(s_sum), (uint32_t)r);
+      out += ld_cluster(at);
+      tie += ld_cluster(at + 4u);
+    }
+    ptx::cluster_sync();                                 // nobody leaves while its counts are read
   }
-  for (int base = s0; base < s1; base += 32) {
-    const int x = kind(base + lane);
-    const uint32_t below = (1u << lane) - 1u, tied = __ballot_sync(0xffffffffu, x == 1);
-    const bool stays = x == 2 || (x == 1 && tie + __popc(tied & below) < need);
-    const uint32_t bal = __ballot_sync(0xffffffffu, stays);
-    if (stays) kept[out + __popc(bal & below)] = base + lane;
-    out += __popc(bal);
-    tie += __popc(tied);
+  out += __reduce_add_sync(0xffffffffu, lane < warp ? s_more[lane < WARPS ? lane : 0] : 0);
+  tie += __reduce_add_sync(0xffffffffu, lane < warp ? s_ties[lane < WARPS ? lane : 0] : 0);
+  out += min(tie, ties);
+  const uint32_t below = (1u << lane) - 1u;
+  const bool all = tie + equal <= ties;                  // of this warp's ties; else none or some
+  if (all || tie >= ties || equal == 0) {
+    const uint32_t from = all ? least : least + 1u;      // (least is kStays only where all of them do)
+    each([&](uint32_t x, int at) {
+      const uint32_t bal = __ballot_sync(0xffffffffu, x >= from);
+      if (x >= from) kept[out + __popc(bal & below)] = at + lane;
+      out += __popc(bal);
+    });
+  } else {
+    each([&](uint32_t x, int at) {
+      const uint32_t tied = __ballot_sync(0xffffffffu, x == least);
+      const bool stays = x > least || (x == least && tie + __popc(tied & below) < ties);
+      const uint32_t bal = __ballot_sync(0xffffffffu, stays);
+      if (stays) kept[out + __popc(bal & below)] = at + lane;
+      out += __popc(bal);
+      tie += __popc(tied);
+    });
   }
+}
+
+template <int PER, int THREADS>
+cudaError_t launch_select(const hbsa_select_keys_args& a, int ctas, cudaStream_t stream) {
+  cudaLaunchAttribute attr[1] = {};
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)ctas;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(a.batch * a.nhead_k * ctas));
+  cfg.blockDim = dim3(THREADS);
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = ctas > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, select_keys_kernel<PER, THREADS>, a, ctas);
 }
 
 // ------------------------------------------------------------------------------------------------------------------
 // Compact: kept positions ascend, so row j comes from row kept[j] >= j, and writing rows [c, d) touches no row that a later chunk still
 // reads.  A CTA takes one slice of the columns of one (sequence, kv-head), of K or of V, chunk by chunk: the rows of the next
-// chunk are read, all threads meet, then the rows of this one are written.
+// chunk are read (their positions one chunk before), all threads meet, then the rows of this one are written.
+// Bound by latency where there are few sequences, by memory otherwise: slices of 64 bytes, so that there are enough CTAs to have 40 KB an SM
+// on their way.
 struct CompactParams {
   void* cache[2];
   Rows4 rows[2];
@@ -221,54 +374,66 @@ struct CompactParams {
   long long table_stride;
   float* weights;
   long long weights_s[2];
-  int num_pages, page, capacity, batch, heads, units, budget;
+  FastDiv page;
+  int num_pages, capacity, batch, heads, units, budget;
   int lanes, slices;                     // units of a slice, slices of K and V together
 };
 constexpr int kCompactThreads = 256, kCompactUnroll = 4;
 
 template <typename U> struct Chunk {
   U x[kCompactUnroll];
-  long long to[kCompactUnroll];          // offset in units, < 0: nothing moves
+  int to[kCompactUnroll];                // where it goes: position (weights) or page, -1: nothing moves
 };
 
-template <typename U, typename Load, typename Store>
-__device__ __forceinline__ void compact_rows(int n, int row, int rows, Load load, Store store) {
+// `next`: reads the positions of a chunk that load takes one call later.
+template <typename U, typename Next, typename Load, typename Store>
+__device__ __forceinline__ void compact_rows(int n, int row, int rows, Next next, Load load, Store store) {
   Chunk<U> a, b;
   const int step = rows * kCompactUnroll;
+  next(row);
   load(a, row);
   for (int c = 0; c < n; c += 2 * step) {
     load(b, c + step + row);
     __syncthreads();
-    store(a);
+    store(a, c + row);
     load(a, c + 2 * step + row);
     __syncthreads();
-    store(b);
+    store(b, c + step + row);
   }
 }
 
 template <typename U>
-__global__ void __launch_bounds__(kCompactThreads) compact_kernel(const __grid_constant__ CompactParams P) {
+__global__ void __launch_bounds__(kCompactThreads, 4) compact_kernel(const __grid_constant__ CompactParams P) {
   const int parts = P.slices + (P.weights != nullptr ? 1 : 0);
   const int part = blockIdx.x % parts, bh = blockIdx.x / parts, b = bh / P.heads, h = bh % P.heads;
   const int len = cut(P.lens[b], P.capacity), n = min(cut(P.kept_lens[b], P.budget), len);
   const int32_t* kept = P.kept + (long long)bh * P.budget;
   const int32_t* table = P.table + b * P.table_stride;
+  int src[kCompactUnroll];               // of the chunk that is read next
   if (part == P.slices) {                // the weights: moved alike, zero behind
     float* w = P.weights + b * P.weights_s[0] + h * P.weights_s[1];
+    auto next = [&](int j0) {
+#pragma unroll
+      for (int e = 0; e < kCompactUnroll; ++e) {
+        const int j = j0 + e * kCompactThreads;
+        src[e] = j < n ? kept[j] : -1;
+      }
+    };
     auto load = [&](Chunk<float>& c, int j0) {
 #pragma unroll
       for (int e = 0; e < kCompactUnroll; ++e) {
-        const int j = j0 + e * kCompactThreads, src = j < n ? kept[j] : -1;
-        c.to[e] = src > j && src < len ? j : -1;
-        if (c.to[e] >= 0) c.x[e] = w[src];
+        const int j = j0 + e * kCompactThreads;
+        c.to[e] = src[e] > j && src[e] < len ? j : -1;
+        if (c.to[e] >= 0) c.x[e] = w[src[e]];
       }
+      next(j0 + kCompactUnroll * kCompactThreads);
     };
-    auto store = [&](const Chunk<float>& c) {
+    auto store = [&](const Chunk<float>& c, int) {
 #pragma unroll
       for (int e = 0; e < kCompactUnroll; ++e)
         if (c.to[e] >= 0) w[c.to[e]] = c.x[e];
     };
-    compact_rows<float>(n, threadIdx.x, kCompactThreads, load, store);
+    compact_rows<float>(n, threadIdx.x, kCompactThreads, next, load, store);
     __syncthreads();
     for (int j = n + threadIdx.x; j < len; j += kCompactThreads) w[j] = 0.f;
     return;
@@ -277,27 +442,40 @@ __global__ void __launch_bounds__(kCompactThreads) compact_kernel(const __grid_c
   const int rows = kCompactThreads / P.lanes;
   const Rows4 s = P.rows[which];
   U* const base = static_cast<U*>(P.cache[which]) + h * s.s[2] + unit * s.s[3];
-  const bool mine = unit < P.units;
+  const int mine = unit < P.units ? n : 0;
+  auto next = [&](int j0) {
+#pragma unroll
+    for (int e = 0; e < kCompactUnroll; ++e) {
+      const int j = j0 + e * rows;
+      src[e] = j < mine ? kept[j] : -1;
+    }
+  };
   auto load = [&](Chunk<U>& c, int j0) {
 #pragma unroll
     for (int e = 0; e < kCompactUnroll; ++e) {
-      const int j = j0 + e * rows, src = mine && j < n ? kept[j] : -1;
+      const int j = j0 + e * rows;
       c.to[e] = -1;
-      if (src > j && src < len) {
-        const int from = table[src / P.page], to = table[j / P.page];
+      if (src[e] > j && src[e] < len) {
+        int slot_from;
+        const int from = table[P.page.split(src[e], slot_from)], to = table[P.page.quotient(j)];
         if (from >= 0 && from < P.num_pages && to >= 0 && to < P.num_pages) {
-          c.x[e] = base[from * s.s[0] + src % P.page * s.s[1]];
-          c.to[e] = to * s.s[0] + j % P.page * s.s[1];
+          c.x[e] = base[from * s.s[0] + slot_from * s.s[1]];
+          c.to[e] = to;
         }
       }
     }
+    next(j0 + kCompactUnroll * rows);
   };
-  auto store = [&](const Chunk<U>& c) {
+  auto store = [&](const Chunk<U>& c, int j0) {
 #pragma unroll
     for (int e = 0; e < kCompactUnroll; ++e)
-      if (c.to[e] >= 0) base[c.to[e]] = c.x[e];
+      if (c.to[e] >= 0) {
+        int slot;
+        P.page.split(j0 + e * rows, slot);
+        base[c.to[e] * s.s[0] + slot * s.s[1]] = c.x[e];
+      }
   };
-  compact_rows<U>(n, threadIdx.x / P.lanes, rows, load, store);
+  compact_rows<U>(n, threadIdx.x / P.lanes, rows, next, load, store);
 }
 
 int element_bytes(int dtype) { return dtype == HBSA_DTYPE_F32 ? 4 : 2; }
@@ -348,8 +526,7 @@ int hbsa_append_to_cache(const hbsa_append_args* a, void* stream) {
   const bool wide = c.headdim * bytes % 16 == 0 && wide_rows(c.k, c.k_stride, 4, bytes) && wide_rows(c.v, c.v_stride, 4, bytes) &&
                     wide_rows(a->k, a->k_stride, 3, bytes) && wide_rows(a->v, a->v_stride, 3, bytes);
   const int per = wide ? 16 / bytes : 1;                 // elements of a unit
-  AppendParams P;
-  memset(&P, 0, sizeof(P));
+  AppendParams P = {};
   P.k = a->k;
   P.v = a->v;
   P.k_cache = c.k;
@@ -369,7 +546,7 @@ int hbsa_append_to_cache(const hbsa_append_args* a, void* stream) {
   P.new_lens = a->new_lens;
   P.status = a->status;
   P.num_pages = c.num_pages;
-  P.page = c.page_size;
+  P.page = FastDiv(c.page_size);
   P.capacity = c.max_pages * c.page_size;
   P.batch = c.batch;
   P.heads = c.nhead_k;
@@ -391,12 +568,25 @@ int hbsa_select_keys(const hbsa_select_keys_args* a, void* stream) {
   if (a->struct_bytes != sizeof(*a)) return set_last_error("hbsa_select_keys_args.struct_bytes does not match this library"), HBSA_ERR_STRUCT;
   if (!a->key_weights || !a->lens || !a->kept || !a->kept_lens) return set_last_error("key_weights, lens, kept and kept_lens must not be NULL"), HBSA_ERR_NULL;
   if (a->batch <= 0 || a->nhead_k <= 0 || a->max_len <= 0 || a->budget <= 0) return set_last_error("batch, nhead_k, max_len and budget must be positive"), HBSA_ERR_SHAPE;
-  if (a->max_len > INT32_MAX - 4096) return set_last_error("max_len does not fit 31 bits"), HBSA_ERR_SHAPE;
+  if (a->max_len > INT32_MAX - 16384) return set_last_error("max_len does not fit 31 bits"), HBSA_ERR_SHAPE;
   if (a->n_sink < 0 || a->n_recent < 0 || (int64_t)a->n_sink + a->n_recent > a->budget)
     return set_last_error("n_sink and n_recent must not be negative, and together not above budget"), HBSA_ERR_SHAPE;
   if ((int64_t)a->batch * a->nhead_k > INT32_MAX / 64) return set_last_error("batch * nhead_k is too large"), HBSA_ERR_SHAPE;
-  select_keys_kernel<<<(unsigned)(a->batch * a->nhead_k), kSelectThreads, 0, static_cast<cudaStream_t>(stream)>>>(*a);
-  return launched("hbsa_select_keys");
+  // CTAs of a row: more than one where there are SMs for them and everyone keeps 4096 positions (128 rows of up to 32768 by two CTAs each,
+  // two on an SM, took 34 us, by one 25), or where one cannot hold them.
+  const long long rows = (long long)a->batch * a->nhead_k, places = sm100_sm_count();
+  int ctas = 1;
+  while (ctas < 8 && rows * ctas * 2 <= places && a->max_len / (2 * ctas) >= 4096) ctas *= 2;
+  while (ctas < 8 && a->max_len > ctas * 32768) ctas *= 2;
+  const int run = ((a->max_len + ctas - 1) / ctas + 31) & ~31;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  cudaError_t e;
+  if (run <= 2048) e = launch_select<8, 256>(*a, ctas, st);
+  else if (run <= 8192) e = launch_select<8, 1024>(*a, ctas, st);
+  else if (run <= 32768) e = launch_select<32, 1024>(*a, ctas, st);
+  else e = launch_select<0, 1024>(*a, ctas, st);
+  if (e != cudaSuccess) return set_last_error("hbsa_select_keys: %s", cudaGetErrorString(e)), (int)e;
+  return 0;
 }
 
 int hbsa_compact_cache(const hbsa_compact_args* a, void* stream) {
@@ -410,8 +600,7 @@ int hbsa_compact_cache(const hbsa_compact_args* a, void* stream) {
   const int bytes = element_bytes(c.dtype);
   const bool wide = c.headdim * bytes % 16 == 0 && wide_rows(c.k, c.k_stride, 4, bytes) && wide_rows(c.v, c.v_stride, 4, bytes);
   const int per = wide ? 16 / bytes : 1;
-  CompactParams P;
-  memset(&P, 0, sizeof(P));
+  CompactParams P = {};
   P.cache[0] = c.k;
   P.cache[1] = c.v;
   for (int i = 0; i < 4; ++i) {
@@ -427,13 +616,13 @@ int hbsa_compact_cache(const hbsa_compact_args* a, void* stream) {
   P.weights_s[0] = a->weights_stride[0];
   P.weights_s[1] = a->weights_stride[1];
   P.num_pages = c.num_pages;
-  P.page = c.page_size;
+  P.page = FastDiv(c.page_size);
   P.capacity = c.max_pages * c.page_size;
   P.batch = c.batch;
   P.heads = c.nhead_k;
   P.units = c.headdim / per;
   P.budget = a->budget;
-  P.lanes = wide ? 8 : 32;
+  P.lanes = wide ? 4 : 32;
   while (wide && P.lanes > 1 && P.lanes >= 2 * P.units) P.lanes /= 2;
   P.slices = 2 * ((P.units + P.lanes - 1) / P.lanes);
   const unsigned grid = (unsigned)(c.batch * c.nhead_k) * (unsigned)(P.slices + (P.weights ? 1 : 0));

@@ -145,6 +145,23 @@ __device__ __forceinline__ int sample_of_block(const int32_t* __restrict__ cnb, 
   return lo;
 }
 
+// Division of 0 <= n < 2^31 by a number known on the host, by multiplication (Granlund and Montgomery, PLDI 1994, figure 4.1):
+// n / d = (n + (n m >> 32)) >> s with s = ceil(log2 d), m = floor(2^32 (2^s - d) / d) + 1; the sum stays below 2^32 for such n.
+struct FastDiv {
+  uint32_t d, m;
+  int s;
+  __host__ FastDiv(int divisor = 1) : d((uint32_t)divisor), s(0) {
+    while ((1ull << s) < d) ++s;
+    m = (uint32_t)(((1ull << 32) * ((1ull << s) - d)) / d + 1);
+  }
+  __device__ __forceinline__ int quotient(int n) const { return (int)(((uint32_t)n + __umulhi((uint32_t)n, m)) >> s); }
+  __device__ __forceinline__ int split(int n, int& rest) const {
+    const int q = quotient(n);
+    rest = n - q * (int)d;
+    return q;
+  }
+};
+
 // Raises a kernel's dynamic shared memory limit once per device instead of before every launch (one static object per kernel;
 // racing callers set the same value).
 struct SmemOptIn {

@@ -616,7 +616,7 @@ PyObject* py_select(PyObject*, PyObject* const* o, Py_ssize_t n) {
   int64_t budget, sink, recent;
   const at::Tensor *w = get_tensor(o[0], &c.dev), *lens = c.int32(o[1], 1);
   if (!w || !lens || wants_gradient(w) || !get_int(o[2], &budget) || !get_int(o[3], &sink) || !get_int(o[4], &recent)) Py_RETURN_NONE;
-  if (w->scalar_type() != at::kFloat || w->dim() != 3 || w->numel() == 0 || w->stride(2) != 1 || w->size(2) >= INT32_MAX - 4095 || w->size(0) > INT32_MAX || w->size(1) > INT32_MAX ||
+  if (w->scalar_type() != at::kFloat || w->dim() != 3 || w->numel() == 0 || w->stride(2) != 1 || w->size(2) > INT32_MAX - 16384 || w->size(0) > INT32_MAX || w->size(1) > INT32_MAX ||
       lens->size(0) != w->size(0) || !lens->is_contiguous())
     Py_RETURN_NONE;
   if (budget <= 0 || sink < 0 || recent < 0 || budget > INT32_MAX || sink > budget || recent > budget || sink + recent > budget) Py_RETURN_NONE;

@@ -263,7 +263,7 @@ def select_keys(key_weights, cache_lens, budget, n_sink=0, n_recent=0):
     _same_device(key_weights, cache_lens)
     _refuse_gradients("select_keys", key_weights)
     assert key_weights.dtype == torch.float32 and key_weights.ndim == 3 and key_weights.shape[2] > 0, "key_weights must be float32 (batch, nhead_k, positions)"
-    assert key_weights.shape[2] < 2 ** 31 - 4096, "the positions must fit 31 bits"
+    assert key_weights.shape[2] < 2 ** 31 - 16384, "the positions must fit 31 bits"
     assert cache_lens.shape == key_weights.shape[:1] and not cache_lens.is_floating_point(), "cache_lens must be an integer tensor of length batch"
     assert budget > 0 and n_sink >= 0 and n_recent >= 0 and n_sink + n_recent <= budget, \
         "budget must be positive, n_sink and n_recent not negative and together not above budget"
