@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ App
 // ------------------------------------------------------------------------------------------------------------------
 // Select: radix select of the smallest weight that stays, then one pass that writes positions in order.  The digits are 11 bits of the distance
 // from the smallest weight above zero (or, where all of those stay, from the smallest of the rest): that keeps keys that nobody has looked at
-// out of the counts, where they would meet in one bin, and spreads weights of one size over many.  A cluster of 1 to 8 CTAs per row; counts
+// out of the counts, where they would meet in one bin, and spreads weights of one size over many.  A cluster of 1 to 4 CTAs per row; counts
 // are exchanged through distributed shared memory.  Every warp has its run of positions, in registers where they fit, as numbers that tell by
 // themselves whether the position competes; where they do not fit, they are read again for every pass.  Bound by the instructions of its
 // passes (23.7 us for 128 rows of 16384 to 32768, 35 us while every pass compared positions): memory is busy for the first one only.
@@ -572,12 +572,12 @@ int hbsa_select_keys(const hbsa_select_keys_args* a, void* stream) {
   if (a->n_sink < 0 || a->n_recent < 0 || (int64_t)a->n_sink + a->n_recent > a->budget)
     return set_last_error("n_sink and n_recent must not be negative, and together not above budget"), HBSA_ERR_SHAPE;
   if ((int64_t)a->batch * a->nhead_k > INT32_MAX / 64) return set_last_error("batch * nhead_k is too large"), HBSA_ERR_SHAPE;
-  // CTAs of a row: more than one where there are SMs for them and everyone keeps 4096 positions (128 rows of up to 32768 by two CTAs each,
-  // two on an SM, took 34 us, by one 25), or where one cannot hold them.
+  // CTAs of a row: more than one where there are SMs for them and a CTA would hold more than 8192 positions, or where one cannot hold them.
+  // 16 rows of 32768 by 1, 2, 4 and 8 CTAs: 22.8, 21.8, 17.0 and 47 us (clusters of eight full SMs do not find their places at once); 16 of
+  // 9000 by 1 and 2: 16.7 and 13.7 us; 8 of 8192 by 1 and 2: 9.9 and 13.3 us.
   const long long rows = (long long)a->batch * a->nhead_k, places = sm100_sm_count();
   int ctas = 1;
-  while (ctas < 8 && rows * ctas * 2 <= places && a->max_len / (2 * ctas) >= 4096) ctas *= 2;
-  while (ctas < 8 && a->max_len > ctas * 32768) ctas *= 2;
+  while (ctas < 4 && a->max_len > ctas * (rows * ctas * 2 <= places ? 8192 : 32768)) ctas *= 2;
   const int run = ((a->max_len + ctas - 1) / ctas + 31) & ~31;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e;
