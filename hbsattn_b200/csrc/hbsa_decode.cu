@@ -101,17 +101,35 @@ __global__ void __launch_bounds__(kGenThreads) decode_generic_kernel(const __gri
   const T* const K = static_cast<const T*>(P.k);
   const T* const V = static_cast<const T*>(P.v);
 
-  // the head dimension beyond headdim stays zero
-  for (int i = tid; i < kDecodeTile * KS; i += kGenThreads) sK[i] = 0.f;
-  for (int i = tid; i < kDecodeTile * DP; i += kGenThreads) sV[i] = 0.f;
+  if (P.headdim < DP) {                                // the columns beyond headdim stay zero
+    for (int i = tid; i < kDecodeTile * KS; i += kGenThreads) sK[i] = 0.f;
+    for (int i = tid; i < kDecodeTile * DP; i += kGenThreads) sV[i] = 0.f;
+  }
   for (long long t = walk.start; t < walk.end;) {
     const DecodeRow r = decode_row_at(P, walk, t, blockIdx.x);
     if (t == walk.start && tid == 0) decode_note_start(P, r);
     t += r.tiles;
     const int head0 = r.hk * P.group + r.chunk * P.chunk_heads;
     const int heads = min(P.chunk_heads, P.group - r.chunk * P.chunk_heads);
+    // threads 0-63: position and place of a key of the tile, found while the tile before is worked on
+    int pos = -1, page = 0, slot = 0;
+    auto look_up = [&](int tile) {
+      if (tid >= kDecodeTile) return;
+      pos = tile * kDecodeTile + tid;
+      if (P.mask != nullptr) {
+        pos = decode_piece_position(P, r, pos / P.unit);
+        if (pos >= 0) pos += tid % P.unit;
+      }
+      if (pos >= r.len) pos = -1;
+      if (pos >= 0) {
+        const int i = pos / P.page;
+        page = P.table[r.b * P.table_stride + i];
+        slot = pos - i * P.page;
+      }
+    };
+    look_up(r.tile0);
     __syncthreads();
-    for (int i = tid; i < kDecodeHeads * DP; i += kGenThreads) {
+    for (int i = tid; i < (heads + 1) / 2 * 2 * DP; i += kGenThreads) {
       const int h = i / DP, d = i % DP;
       sQ[i] = h < heads && d < P.headdim ? to_f(static_cast<const T*>(P.q)[r.b * P.q_s[0] + (head0 + h) * P.q_s[1] + d * P.q_s[2]]) : 0.f;
     }
@@ -128,15 +146,8 @@ __global__ void __launch_bounds__(kGenThreads) decode_generic_kernel(const __gri
     for (int tile = r.tile0; tile < r.tile0 + r.tiles; ++tile) {
       __syncthreads();                                 // the tile before is used up
       if (tid < kDecodeTile) {
-        int pos = tile * kDecodeTile + tid;
-        if (P.mask != nullptr) {
-          pos = decode_piece_position(P, r, pos / P.unit);
-          if (pos >= 0) pos += tid % P.unit;
-        }
-        if (pos >= r.len) pos = -1;
         long long k_at = -1, v_at = -1;
         if (pos >= 0) {
-          const int page = P.table[r.b * P.table_stride + pos / P.page], slot = pos % P.page;
           if (page >= 0 && page < P.num_pages) {
             k_at = page * P.k_s[0] + slot * P.k_s[1] + r.hk * P.k_s[2];
             v_at = page * P.v_s[0] + slot * P.v_s[1] + r.hk * P.v_s[2];
@@ -148,10 +159,12 @@ __global__ void __launch_bounds__(kGenThreads) decode_generic_kernel(const __gri
         sh.k_at[tid] = k_at;
         sh.v_at[tid] = v_at;
       }
+      if (tile + 1 < r.tile0 + r.tiles) look_up(tile + 1);
       __syncthreads();
       const int vecs = P.headdim / VEC;
+#pragma unroll 4
       for (int i = tid; i < kDecodeTile * vecs; i += kGenThreads) {
-        const int key = i / vecs, d = i % vecs * VEC;
+        const int key = i / vecs, d = (i - key * vecs) * VEC;
         const long long ka = sh.k_at[key], va = sh.v_at[key];
         if (VEC > 1) {
           union { uint4 w; T x[16 / sizeof(T)]; } a, b;
@@ -173,7 +186,7 @@ __global__ void __launch_bounds__(kGenThreads) decode_generic_kernel(const __gri
       __syncthreads();
       // scores: thread = (key, every fourth pair of heads)
       {
-        const int key = tid & 63, pos = sh.pos[key];
+        const int key = tid & 63, at = sh.pos[key];
         const bool there = sh.k_at[key] >= 0;
         const float4* kr = reinterpret_cast<const float4*>(sK + key * KS);
         for (int h = 2 * (tid >> 6); h < heads; h += 8) {
@@ -189,8 +202,8 @@ __global__ void __launch_bounds__(kGenThreads) decode_generic_kernel(const __gri
           s1 = there ? s1 * P.scale_log2 : -INFINITY;
           sP[h * kDecodeTile + key] = s0;
           sP[(h + 1) * kDecodeTile + key] = s1;
-          if (P.weights != nullptr && pos >= 0) {
-            float* to = P.sp.scores + ((long long)r.b * P.nhead_q + head0 + h) * P.capacity + pos;
+          if (P.weights != nullptr && at >= 0) {
+            float* to = P.sp.scores + ((long long)r.b * P.nhead_q + head0 + h) * P.capacity + at;
             to[0] = s0;
             if (h + 1 < heads) to[P.capacity] = s1;
           }
@@ -281,25 +294,54 @@ struct DecodeParts {
 constexpr int kJoinThreads = 256;
 constexpr int kJoinMost = 1024;          // CTAs of the main kernel, at most
 
-// CTA (c, y), weights: those of the keys that CTA c of the main kernel has worked on.
-__device__ __forceinline__ void add_weights(const DecodeParams& P, const DecodeCut& cut, const int4 st, int c) {
-  constexpr int WARPS = kJoinThreads / 32;
+// CTA (c, part) of the weights: a quarter of the tiles that CTA c of the main kernel has worked on.  A quarter, because the way to the first
+// position is a chain of loads, and few keys wait behind it: a call of 6 x 301..3001 keys, 8 heads, groups of 3 took 33.8, 29.5, 29.5 and 33.8 us
+// with 1, 2, 4 and 8 parts.
+constexpr int kWeightParts = 4;
+__device__ __forceinline__ void add_weights(const DecodeParams& P, const DecodeCut& cut, const int4 st, int c, int part) {
+  constexpr int WARPS = kJoinThreads / 32, EARLY = 8;
   __shared__ float s_lse[kJoinMost];     // of the group's heads, in the log2 domain
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (st.x < 0) return;
   DecodeWalk walk;
-  walk.start = cut.first(c / P.lanes);
-  walk.end = walk.start + cut.tiles(c / P.lanes);
+  const long long start = cut.first(c / P.lanes), n_tiles = cut.tiles(c / P.lanes);
+  walk.start = start;
+  walk.end = start + n_tiles * (part + 1) / kWeightParts;
   const int hk0 = st.y / P.n_chunk, in_entry = P.mask == nullptr ? st.y : st.y % P.n_chunk;
   walk.entry = P.mask == nullptr ? st.x : st.x * P.nhead_k + hk0;
-  walk.entry_start = walk.start - st.z - (long long)in_entry * st.w;
-  for (long long t = walk.start; t < walk.end;) {
+  walk.entry_start = start - st.z - (long long)in_entry * st.w;
+  for (long long t = start + n_tiles * part / kWeightParts; t < walk.end;) {
     const DecodeRow r = decode_row_at(P, walk, t, c);
     const long long row0 = t - r.tile0, head0 = (long long)r.b * P.nhead_q + r.hk * P.group;
     t += r.tiles;
     if (r.chunk != 0) continue;          // the first chunk's tiles stand for the whole group
+    float* const out = P.weights + r.b * P.weights_s[0] + r.hk * P.weights_s[1];
     for (int h0 = 0; h0 < P.group; h0 += kJoinMost) {
-      const int heads = min(kJoinMost, P.group - h0);
+      const int heads = min(kJoinMost, P.group - h0), last = 2 * (r.tile0 + r.tiles);
+      const float* const scores = P.sp.scores + (head0 + h0) * P.capacity;
+      // half a tile per warp and go; the first one's numbers are on their way while the sums are put together, then the next one's
+      int pos = -1;
+      float old = 0.f, x[EARLY];
+      auto fetch = [&](int i) {
+        pos = -1;
+        if (i < last) {
+          pos = i * 32 + lane;
+          if (P.mask != nullptr) {
+            const int in = pos;
+            pos = decode_piece_position(P, r, in / P.unit);
+            if (pos >= 0) pos += in % P.unit;
+          }
+          if (pos >= r.len) pos = -1;
+        }
+        if (pos >= 0) {
+          old = out[pos];
+#pragma unroll
+          for (int h = 0; h < EARLY; ++h)
+            if (h < heads) x[h] = scores[(long long)h * P.capacity + pos];
+        }
+      };
+      int i = 2 * r.tile0 + warp;
+      fetch(i);
       __syncthreads();
       for (int h = warp; h < heads; h += WARPS) {
         const int chunk = (h0 + h) / P.chunk_heads, head = (h0 + h) % P.chunk_heads;
@@ -309,12 +351,12 @@ __device__ __forceinline__ void add_weights(const DecodeParams& P, const DecodeC
           lse = P.lse[head0 + h0 + h] * kDecodeLog2e;
         } else {
           float mx = -INFINITY, l = 0.f;
-          for (int i = lane; i < parts.n; i += 32) mx = fmaxf(mx, P.sp.part_ml[(parts.at(i) * kDecodeHeads + head) * 2]);
+          for (int k = lane; k < parts.n; k += 32) mx = fmaxf(mx, P.sp.part_ml[(parts.at(k) * kDecodeHeads + head) * 2]);
 #pragma unroll
           for (int s = 16; s > 0; s >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, s));
           const float ref = mx == -INFINITY ? 0.f : mx;
-          for (int i = lane; i < parts.n; i += 32) {
-            const float2 ml = *reinterpret_cast<const float2*>(P.sp.part_ml + (parts.at(i) * kDecodeHeads + head) * 2);
+          for (int k = lane; k < parts.n; k += 32) {
+            const float2 ml = *reinterpret_cast<const float2*>(P.sp.part_ml + (parts.at(k) * kDecodeHeads + head) * 2);
             l += exp2f(ml.x - ref) * ml.y;
           }
 #pragma unroll
@@ -324,73 +366,68 @@ __device__ __forceinline__ void add_weights(const DecodeParams& P, const DecodeC
         if (lane == 0) s_lse[h] = lse;
       }
       __syncthreads();
-      const float* scores = P.sp.scores + (head0 + h0) * P.capacity;
-      float* const out = P.weights + r.b * P.weights_s[0] + r.hk * P.weights_s[1];
-      // half a tile per warp and go
-      for (int i = 2 * r.tile0 + warp; i < 2 * (r.tile0 + r.tiles); i += WARPS) {
-        int pos = i * 32 + lane;
-        if (P.mask != nullptr) {
-          const int in = pos;
-          pos = decode_piece_position(P, r, in / P.unit);
-          if (pos >= 0) pos += in % P.unit;
-        }
-        if (pos < 0 || pos >= r.len) continue;
+      for (; i < last; i += WARPS) {
+        const int at = pos;
         float w = 0.f;
-        const float old = out[pos];
-#pragma unroll 8
-        for (int h = 0; h < heads; ++h) {
-          const float lse = s_lse[h], x = scores[(long long)h * P.capacity + pos];
-          if (lse != -INFINITY) w += exp2f(x - lse);
+        const float before = old;
+        if (at >= 0) {
+#pragma unroll
+          for (int h = 0; h < EARLY; ++h)
+            if (h < heads && s_lse[h] != -INFINITY) w += exp2f(x[h] - s_lse[h]);
         }
-        out[pos] = old + w;
+        fetch(i + WARPS);
+        if (at < 0) continue;
+#pragma unroll 4
+        for (int h = EARLY; h < heads; ++h) {
+          const float lse = s_lse[h], y = scores[(long long)h * P.capacity + at];
+          if (lse != -INFINITY) w += exp2f(y - lse);
+        }
+        out[at] = before + w;
       }
     }
   }
 }
 
-// CTA (j, h): q-head h of the row whose second part is that of CTA j of the main kernel; behind the heads: the weights.  CTA (0, 0) writes
-// the status words.
+// CTA (j, y): first the weights, then q-head y of the row whose second part is that of CTA j of the main kernel.  CTA (0, 0) writes the status words.
 template <typename T>
-__global__ void __launch_bounds__(kJoinThreads) decode_join_kernel(const __grid_constant__ DecodeParams P) {
+__global__ void __launch_bounds__(kJoinThreads, 4) decode_join_kernel(const __grid_constant__ DecodeParams P) {
   __shared__ float s_f[kJoinMost];
   __shared__ float4 s_acc[kJoinThreads];
   __shared__ float s_red[2][kJoinThreads / 32];
-  __shared__ int s_first, s_code;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, j = blockIdx.x, head = blockIdx.y;
-  if (tid == 0) {
-    s_first = 0x7fffffff;
-    s_code = 0;
-  }
+  __shared__ int s_first;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, j = blockIdx.x, parts_y = P.weights != nullptr ? kWeightParts : 0;
+  const int head = (int)blockIdx.y - parts_y;
+  if (tid == 0) s_first = 0x7fffffff;
   pdl_wait();
   const int4 st = P.sp.cta_start[j];
   const DecodeCut cut(*P.sp.total, P.runs);
-  __syncthreads();
-  for (int c = tid; c < P.grid; c += kJoinThreads) {
-    const int code = P.sp.cta_status[2 * c];
-    if (code != HBSA_STATUS_OK) {
-      atomicOr(&s_code, 1 << code);
-      if (code == HBSA_STATUS_CACHE_BOUNDS) atomicMin(&s_first, P.sp.cta_status[2 * c + 1]);
+  int codes = 0;
+  for (int c = tid; c < P.grid; c += kJoinThreads) codes |= 1 << P.sp.cta_status[2 * c];
+  const bool gave_up = __syncthreads_or(codes & (1 << HBSA_STATUS_WAIT_LIMIT)) != 0;
+  if (j == 0 && blockIdx.y == 0) {
+    const bool bounds = __syncthreads_or(codes & (1 << HBSA_STATUS_CACHE_BOUNDS)) != 0;
+    if (bounds)
+      for (int c = tid; c < P.grid; c += kJoinThreads)
+        if (P.sp.cta_status[2 * c] == HBSA_STATUS_CACHE_BOUNDS) atomicMin(&s_first, P.sp.cta_status[2 * c + 1]);
+    __syncthreads();
+    if (tid < kStatusWords) {
+      int w = 0;
+      if (tid == 0) w = gave_up ? (int)HBSA_STATUS_WAIT_LIMIT : bounds ? (int)HBSA_STATUS_CACHE_BOUNDS : (int)HBSA_STATUS_OK;
+      if (tid == 1 && !gave_up && bounds) w = s_first;
+      P.sp.status[tid] = w;
     }
-  }
-  __syncthreads();
-  const bool gave_up = (s_code & (1 << HBSA_STATUS_WAIT_LIMIT)) != 0;
-  if (j == 0 && head == 0 && tid < kStatusWords) {
-    int w = 0;
-    if (tid == 0) w = gave_up ? (int)HBSA_STATUS_WAIT_LIMIT : s_code != 0 ? (int)HBSA_STATUS_CACHE_BOUNDS : (int)HBSA_STATUS_OK;
-    if (tid == 1 && !gave_up && s_code != 0) w = s_first;
-    P.sp.status[tid] = w;
   }
   if (gave_up) {                         // nobody shall take the output for one
     const long long n = (long long)P.batch * P.nhead_q * P.headdim, step = (long long)gridDim.x * gridDim.y * kJoinThreads;
-    for (long long i = ((long long)head * gridDim.x + j) * kJoinThreads + tid; i < n; i += step) {
+    for (long long i = ((long long)blockIdx.y * gridDim.x + j) * kJoinThreads + tid; i < n; i += step) {
       const long long row = i / P.headdim, b = row / P.nhead_q, h = row % P.nhead_q, d = i % P.headdim;
       static_cast<T*>(P.o)[b * P.o_s[0] + h * P.o_s[1] + d * P.o_s[2]] = from_f<T>(NAN);
       if (d == 0 && P.lse != nullptr) P.lse[row] = NAN;
     }
     return;
   }
-  if (head == P.chunk_heads) {
-    add_weights(P, cut, st, j);
+  if (head < 0) {
+    add_weights(P, cut, st, j, (int)blockIdx.y);
     return;
   }
   if (st.x < 0 || st.z == 0) return;
@@ -632,7 +669,7 @@ int hbsa_paged_attention(const hbsa_paged_attention_args* args, void* stream_) {
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)P.grid, (unsigned)(P.chunk_heads + (P.weights ? 1 : 0)));
+  cfg.gridDim = dim3((unsigned)P.grid, (unsigned)(P.chunk_heads + (P.weights ? hbsa::kWeightParts : 0)));
   cfg.blockDim = dim3(hbsa::kJoinThreads);
   cfg.stream = stream;
   cfg.attrs = attr;

@@ -58,17 +58,22 @@ struct DecodeParams {
   int grid, lanes, runs;     // G = lanes * runs
 };
 
+// a / b of numbers that are not negative; nearly always both fit 32 bits, where the division is several times shorter.
+__device__ __forceinline__ long long quotient(long long a, long long b) {
+  return (unsigned long long)(a | b) >> 32 == 0 ? (long long)((uint32_t)a / (uint32_t)b) : a / b;
+}
+
 // The cut of `total` tiles into `grid` runs: the first `rem` have base + 1 tiles, the others base.
 struct DecodeCut {
   long long base;
   int rem;
-  __device__ __forceinline__ DecodeCut(long long total, int grid) : base(total / grid), rem((int)(total - total / grid * grid)) {}
+  __device__ __forceinline__ DecodeCut(long long total, int grid) : base(quotient(total, grid)), rem((int)(total - base * grid)) {}
   __device__ __forceinline__ long long first(int c) const { return c * base + min(c, rem); }
   __device__ __forceinline__ int tiles(int c) const { return (int)base + (c < rem ? 1 : 0); }
   // the run that has tile t
   __device__ __forceinline__ int owner(long long t) const {
     const long long front = rem * (base + 1);
-    return t < front ? (int)(t / (base + 1)) : rem + (int)((t - front) / base);
+    return t < front ? (int)quotient(t, base + 1) : rem + (int)quotient(t - front, base);
   }
 };
 
@@ -146,7 +151,7 @@ __device__ __forceinline__ DecodeRow decode_row_at(const DecodeParams& P, Decode
     walk.entry_start += (long long)tiles * rows;
     tiles = decode_row_tiles(P, ++walk.entry);
   }
-  const int in_entry = (int)((t - walk.entry_start) / tiles);
+  const int in_entry = (int)quotient(t - walk.entry_start, tiles);
   const long long row0 = walk.entry_start + (long long)in_entry * tiles;
   r.entry = walk.entry;
   r.b = P.mask == nullptr ? walk.entry : walk.entry / P.nhead_k;
