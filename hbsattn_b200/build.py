@@ -26,7 +26,7 @@ HOST_SOURCE = os.path.join(CSRC, "hbsa_host.cpp")
 STRICT_LIB_PATH = os.path.join(PKG_DIR, "libhbsattn_b200_strict.so")
 SOURCES = ["hbsa_api.cu", "hbsa_schedule.cu", "hbsa_fwd_generic.cu", "hbsa_fwd_sm100.cu",
            "hbsa_bwd_sm100.cu", "hbsa_bwd_generic.cu", "hbsa_static_scratch.cu",
-           "hbsa_cache.cu", "hbsa_decode.cu", "hbsa_decode_sm100.cu", "hbsa_key_weights.cu", "hbsa_key_weights_sm100.cu"]
+           "hbsa_cache.cu", "hbsa_decode.cu", "hbsa_decode_sm100.cu", "hbsa_decode_f32.cu", "hbsa_key_weights.cu", "hbsa_key_weights_sm100.cu"]
 HEADERS = ["hbsa_common.cuh", "sm100_ptx.cuh", "sm100_common.cuh", "hbsa_decode.cuh", "hbsa_key_weights.cuh", os.path.join("..", "..", "include", "hbsattn_b200.h")]
 
 

@@ -1,5 +1,5 @@
 // Attention of one new token per sequence over a paged key-value cache: everything but the tensor-core main kernel
-// (hbsa_decode_sm100.cu).  For every sequence b and q-head h, over the positions j < len_b in active blocks:
+// (hbsa_decode_sm100.cu) and the one for fp32 (hbsa_decode_f32.cu).  For every sequence b and q-head h, over the positions j < len_b in active blocks:
 //     x_j = scale * q . k_j        o = sum_j exp(x_j - lse) v_j        lse = ln sum_j exp x_j
 // and, where wanted, weights[b, kv-head, j] += sum over the heads of the group of exp(x_j - lse).
 //
@@ -511,6 +511,11 @@ cudaError_t launch_generic_of(const DecodeParams& P, bool dependent, cudaStream_
   return vec ? launch_generic<T, 256, VEC>(P, dependent, stream) : launch_generic<T, 256, 1>(P, dependent, stream);
 }
 
+// The main kernel; the generic one where neither is set.
+struct DecodeKind {
+  bool sm100, f32;
+};
+
 size_t align256(size_t x) { return (x + 255) / 256 * 256; }
 
 int gcd(int a, int b) {
@@ -522,9 +527,9 @@ int gcd(int a, int b) {
   return a;
 }
 
-// CTAs of the main kernel: one per SM of the tensor-core kernel, as many as fit of the other.
-int decode_grid(bool sm100, int d_pad) {
-  const int per_sm = sm100 ? 1 : d_pad == 64 ? 4 : d_pad == 128 ? 2 : 1;
+// CTAs of the main kernel: one per SM of the tensor-core kernel, as many as fit of the others.
+int decode_grid(const DecodeKind& kind, int d_pad) {
+  const int per_sm = kind.sm100 ? 1 : kind.f32 ? 2 : d_pad == 64 ? 4 : d_pad == 128 ? 2 : 1;
   const int n = sm100_sm_count() * per_sm;
   return n < kJoinMost ? n : kJoinMost;
 }
@@ -547,7 +552,7 @@ size_t carve_decode(const DecodeParams& P, char* base, DecodeSpace* s, bool own_
 }
 
 // Everything but the launches; also what the workspace's size comes from (need_tensors false: pointers may be missing).
-int make_decode(const hbsa_paged_attention_args* a, bool need_tensors, DecodeParams* P, bool* sm100, size_t* bytes) {
+int make_decode(const hbsa_paged_attention_args* a, bool need_tensors, DecodeParams* P, DecodeKind* kind, size_t* bytes) {
   if (!a) return set_last_error("args is NULL"), HBSA_ERR_NULL;
   if (a->struct_bytes != sizeof(*a)) return set_last_error("hbsa_paged_attention_args.struct_bytes does not match this library"), HBSA_ERR_STRUCT;
   const hbsa_cache& c = a->cache;
@@ -590,6 +595,7 @@ int make_decode(const hbsa_paged_attention_args* a, bool need_tensors, DecodePar
   P->weights_s[1] = a->weights_stride[1];
   P->num_pages = c.num_pages;
   P->page = c.page_size;
+  P->page_div = FastDiv(c.page_size);
   P->batch = c.batch;
   P->nhead_q = a->nhead_q;
   P->nhead_k = c.nhead_k;
@@ -605,17 +611,18 @@ int make_decode(const hbsa_paged_attention_args* a, bool need_tensors, DecodePar
   P->debug_stall = sm100_debug_stall();
   const char* why = decode_sm100_ineligible_reason(*a, scale);
   if (need_tensors && a->impl == HBSA_IMPL_SM100 && why) return set_last_error("the tensor-core kernel cannot run this problem: %s", why), HBSA_ERR_UNSUPPORTED;
-  *sm100 = !why && a->impl != HBSA_IMPL_GENERIC;
-  const int most_heads = *sm100 && P->d_pad == 256 ? 16 : kDecodeHeads;
+  kind->sm100 = !why && a->impl != HBSA_IMPL_GENERIC;
+  kind->f32 = decode_f32_eligible(*a);
+  const int most_heads = kind->f32 ? (P->d_pad == 256 ? 4 : 8) : kind->sm100 && P->d_pad == 256 ? 16 : kDecodeHeads;
   P->n_chunk = (P->group + most_heads - 1) / most_heads;
   P->chunk_heads = (P->group + P->n_chunk - 1) / P->n_chunk;
   P->unit = kDecodeTile;
-  if (*sm100) P->unit = gcd(P->unit, P->page);
+  if (kind->sm100) P->unit = gcd(P->unit, P->page);
   if (P->mask) P->unit = gcd(P->unit, P->kbs);
   P->pieces_per_block = P->mask ? P->kbs / P->unit : 0;
   P->one_box = P->headdim % 64 == 0;
   P->lanes = P->mask || P->nhead_k % 2 ? 1 : P->nhead_k % 4 ? 2 : 4;
-  P->runs = decode_grid(*sm100, P->d_pad) / P->lanes;
+  P->runs = decode_grid(*kind, P->d_pad) / P->lanes;
   P->grid = P->runs * P->lanes;
   const bool own_lse = a->key_weights && !a->lse;
   *bytes = carve_decode(*P, static_cast<char*>(a->workspace), &P->sp, own_lse);
@@ -637,16 +644,16 @@ extern "C" {
 
 size_t hbsa_paged_attention_workspace_bytes(const hbsa_paged_attention_args* args) {
   hbsa::DecodeParams P;
-  bool sm100;
+  hbsa::DecodeKind kind;
   size_t bytes;
-  return hbsa::make_decode(args, false, &P, &sm100, &bytes) == 0 ? bytes : 0;
+  return hbsa::make_decode(args, false, &P, &kind, &bytes) == 0 ? bytes : 0;
 }
 
 int hbsa_paged_attention(const hbsa_paged_attention_args* args, void* stream_) {
   hbsa::DecodeParams P;
-  bool sm100;
+  hbsa::DecodeKind kind;
   size_t bytes;
-  int rc = hbsa::make_decode(args, true, &P, &sm100, &bytes);
+  int rc = hbsa::make_decode(args, true, &P, &kind, &bytes);
   if (rc != 0) return rc;
   if (args->workspace_bytes < bytes) return hbsa::set_last_error("workspace is smaller than hbsa_paged_attention_workspace_bytes()"), HBSA_ERR_WORKSPACE;
   if ((uintptr_t)args->workspace % 256 != 0) return hbsa::set_last_error("workspace must be 256-byte aligned"), HBSA_ERR_WORKSPACE;
@@ -655,11 +662,11 @@ int hbsa_paged_attention(const hbsa_paged_attention_args* args, void* stream_) {
   cudaError_t e = cudaSuccess;
   const bool masked = P.mask != nullptr;
   if (masked && (e = hbsa::launch_kernel(hbsa::decode_blocks_kernel, (unsigned)((P.batch * P.nhead_k + 7) / 8), 256, 0, false, stream, P)) != cudaSuccess) return failed(e);
-  if (sm100) {
+  if (kind.sm100) {
     const char* text = "";
     rc = hbsa::launch_decode_sm100(P, *args, masked, stream, &text);
     if (rc != 0) return hbsa::set_last_error("hbsa_paged_attention: %s", text), rc;
-  } else if ((e = hbsa::launch_decode_generic(P, args->cache.dtype, masked, stream)) != cudaSuccess) {
+  } else if ((e = kind.f32 ? hbsa::launch_decode_f32(P, masked, stream) : hbsa::launch_decode_generic(P, args->cache.dtype, masked, stream)) != cudaSuccess) {
     return failed(e);
   }
   auto join = args->cache.dtype == HBSA_DTYPE_BF16  ? hbsa::decode_join_kernel<__nv_bfloat16>

@@ -46,6 +46,7 @@ struct DecodeParams {
   float* lse;                // the caller's, or the workspace's, or NULL
   float* weights;
   long long weights_s[2];
+  FastDiv page_div;
   int num_pages, page, capacity, batch, nhead_q, nhead_k, group, headdim, d_pad;
   int n_chunk, chunk_heads;  // chunks of a group, q-heads of every chunk but perhaps the last
   int kbs, num_k_block;
@@ -201,6 +202,8 @@ __device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.laun
 
 const char* decode_sm100_ineligible_reason(const hbsa_paged_attention_args& a, float scale);
 // The main kernel: every row that one CTA has alone is written, the others leave their parts.
+bool decode_f32_eligible(const hbsa_paged_attention_args& a);
+cudaError_t launch_decode_f32(const DecodeParams& P, bool dependent, cudaStream_t stream);
 cudaError_t launch_decode_generic(const DecodeParams& P, int dtype, bool dependent, cudaStream_t stream);
 int launch_decode_sm100(const DecodeParams& P, const hbsa_paged_attention_args& a, bool dependent, cudaStream_t stream, const char** err_text);
 
