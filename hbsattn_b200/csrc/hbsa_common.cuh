@@ -162,6 +162,11 @@ struct FastDiv {
   }
 };
 
+// a / b of numbers that are not negative; nearly always both fit 32 bits, where the division is several times shorter.
+__device__ __forceinline__ long long quotient(long long a, long long b) {
+  return (unsigned long long)(a | b) >> 32 == 0 ? (long long)((uint32_t)a / (uint32_t)b) : a / b;
+}
+
 // Raises a kernel's dynamic shared memory limit once per device instead of before every launch (one static object per kernel;
 // racing callers set the same value).
 struct SmemOptIn {

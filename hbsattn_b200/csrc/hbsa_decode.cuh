@@ -59,11 +59,6 @@ struct DecodeParams {
   int grid, lanes, runs;     // G = lanes * runs
 };
 
-// a / b of numbers that are not negative; nearly always both fit 32 bits, where the division is several times shorter.
-__device__ __forceinline__ long long quotient(long long a, long long b) {
-  return (unsigned long long)(a | b) >> 32 == 0 ? (long long)((uint32_t)a / (uint32_t)b) : a / b;
-}
-
 // The cut of `total` tiles into `grid` runs: the first `rem` have base + 1 tiles, the others base.
 struct DecodeCut {
   long long base;

@@ -4,7 +4,10 @@
 // (hbsa_decode.cu) they say which keys of a cache can go (hbsa_select_keys).
 //
 // This file: the entry point, the preparation kernel, and the CUDA-core kernel for fp32, odd strides and head dimensions.
-// One CTA = 64 keys of one (kv-head, k-block); rows of the active q-blocks are streamed past them, 64 at a time.
+// One cluster = 64 keys of one (kv-head, k-block).  The rows of the active q-blocks stand in one line, which is cut into tiles of 64 that the
+// cluster's CTAs take in turn: thread = 4 keys x 4 rows, whose products it adds up from shared memory.  Bound by the multiplications and the way from
+// tile to tile (barriers, loads): 2 x 4096 tokens, 8 heads of 128, 30 % of the blocks: 579 us, 21 TFLOP/s; one CTA per 64 keys with 4 rows x 1 key a
+// thread took 1160 us, and with few keys (2048 x 2 kv-heads) 516 instead of 62 us.
 #include <string.h>
 
 #include "hbsa_key_weights.cuh"
@@ -52,96 +55,194 @@ __global__ void __launch_bounds__(256) key_weights_prep_kernel(const __grid_cons
 
 struct KeyWeightsStrides { long long q0, q1, q2, k0, k1, k2; };
 
-template <typename T, int DP>
-__global__ void __launch_bounds__(kThreads) key_weights_generic_kernel(const __grid_constant__ KeyWeightsParams P, const T* __restrict__ q, const T* __restrict__ k,
-                                                                       KeyWeightsStrides st) {
-  constexpr int KS = DP + 4;
+constexpr int kList = 1024;                      // q-blocks that are looked at together
+
+// VEC: elements of a 16-byte unit, or 1.
+template <typename T, int DP, int VEC>
+__global__ void __launch_bounds__(kThreads, DP == 256 ? 1 : 2) key_weights_generic_kernel(const __grid_constant__ KeyWeightsParams P, const T* __restrict__ q,
+                                                                                          const T* __restrict__ k, KeyWeightsStrides st, int ctas) {
+  constexpr int KS = DP + 4;                     // rows 4 floats apart modulo 32: 16-byte reads of 8 rows hit all banks
   const Problem& p = P.p;
   if (P.ws.status[0] != HBSA_STATUS_OK) return;
   extern __shared__ __align__(16) float sm[];
   float* const sK = sm;                          // [kKeys][KS]
-  float* const sQ = sK + kKeys * KS;             // [kRows][DP]
-  __shared__ float s_nl[kRows], s_sum[kThreads];
-  const int subs = (p.kbs + kKeys - 1) / kKeys, kb = blockIdx.x / subs, sub = blockIdx.x % subs, hk = blockIdx.y;
+  float* const sQ = sK + kKeys * KS;             // [kRows][KS]
+  __shared__ long long s_at[kRows];              // element offset of a row of q, or -1
+  __shared__ float s_nl[kRows], s_sum[16][kKeys];
+  __shared__ int s_pos[kRows], s_list[kList], s_count[kThreads / 32];
+  const int subs = (p.kbs + kKeys - 1) / kKeys, item = blockIdx.x / ctas, rank = blockIdx.x - item * ctas, kb = item / subs, sub = item % subs, hk = blockIdx.y;
   const int b = sample_of_block(P.ws.cnk, p.batch, kb);
   const int k_begin = p.cu_k[b], k_len = p.cu_k[b + 1] - k_begin, q_begin = p.cu_q[b], q_len = p.cu_q[b + 1] - q_begin, off = k_len - q_len;
   const int blk0 = (kb - P.ws.cnk[b]) * p.kbs, k0 = blk0 + sub * kKeys, n_keys = min(kKeys, min(blk0 + p.kbs, k_len) - k0);
-  if (n_keys <= 0) return;
-  const int tid = threadIdx.x, key = tid & 63, part = tid >> 6;
-  for (int i = tid; i < kKeys * DP; i += kThreads) {
-    const int r = i / DP, d = i % DP;
-    sK[r * KS + d] = r < n_keys && d < p.headdim ? to_f(k[(long long)(k_begin + k0 + r) * st.k0 + hk * st.k1 + d * st.k2]) : 0.f;
-  }
-  const int qb0 = P.ws.cnq[b], n_qb = P.ws.cnq[b + 1] - qb0;
-  float sum = 0.f;
-  for (int i = 0; i < n_qb; ++i) {
-    bool on;
-    if (p.csr_ptr != nullptr) {
-      const long long row = (long long)hk * p.num_q_block + qb0 + i;
-      const int e1 = p.csr_ptr[row + 1], e = lower_bound_i32(p.csr_idx, p.csr_ptr[row], e1, kb);
-      on = e < e1 && p.csr_idx[e] == kb;
-    } else {
-      on = p.mask[hk * p.mask_s0 + (long long)(qb0 + i) * p.mask_s1 + (long long)kb * p.mask_s2] != 0;
-    }
-    const int row_end = min((i + 1) * p.qbs, q_len);
-    if (!on || (p.causal && row_end - 1 + off < k0)) continue;       // uniform over the CTA
-    const int n_rows = (row_end - i * p.qbs) * p.group;              // (token, head) pairs, heads innermost
-    for (int r0 = 0; r0 < n_rows; r0 += kRows) {
-      __syncthreads();
-      for (int j = tid; j < kRows * DP; j += kThreads) {
-        const int r = r0 + j / DP, d = j % DP;
-        const long long tok = q_begin + i * p.qbs + r / p.group;
-        sQ[j] = r < n_rows && d < p.headdim ? to_f(q[tok * st.q0 + (hk * p.group + r % p.group) * st.q1 + d * st.q2]) : 0.f;
-      }
-      if (tid < kRows) {
-        const int r = r0 + tid;
-        const int h = hk * p.group + r % p.group;
-        s_nl[tid] = r < n_rows ? P.sp.neg_lse[(((long long)(h >> P.gp_shift) * p.num_q_block + qb0 + i) * p.qbs + r / p.group) * P.gp + (h & (P.gp - 1))] : -INFINITY;
-      }
-      __syncthreads();
-      float tile_sum = 0.f;
-      for (int rr = part * 16; rr < part * 16 + 16; rr += 4) {
-        float s[4] = {0.f, 0.f, 0.f, 0.f};
-        const float4* kr = reinterpret_cast<const float4*>(sK + key * KS);
+  if (n_keys <= 0) return;                       // the whole cluster
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, tx = tid & 15, ty = tid >> 4;
+  // 64 rows of K or Q: at(row) is the row's offset, or -1
+  auto load = [&](float* to, const T* from, long long stride, auto&& at) {
+    const int units = DP / VEC, there = p.headdim / VEC;
 #pragma unroll 4
-        for (int d = 0; d < DP / 4; ++d) {
-          const float4 x = kr[d];
+    for (int i = tid; i < 64 * units; i += kThreads) {
+      const int r = i / units, u = i % units;
+      const long long row = at(r);
+      float* const dst = to + r * KS + u * VEC;
+      const bool on = row >= 0 && u < there;
+      if (VEC > 1) {
+        union { uint4 w; T x[16 / sizeof(T)]; } in;
+        in.w = make_uint4(0u, 0u, 0u, 0u);
+        if (on) in.w = *reinterpret_cast<const uint4*>(from + row + u * VEC);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float4 y = *reinterpret_cast<const float4*>(sQ + (rr + e) * DP + 4 * d);
-            s[e] = fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, fmaf(x.w, y.w, s[e]))));
+        for (int e = 0; e < VEC; ++e) dst[e] = to_f(in.x[e]);
+      } else {
+        dst[0] = on ? to_f(from[row + u * stride]) : 0.f;
+      }
+    }
+  };
+  load(sK, k, st.k2, [&](int r) { return r < n_keys ? (long long)(k_begin + k0 + r) * st.k0 + hk * st.k1 : -1ll; });
+  const int qb0 = P.ws.cnq[b], n_qb = P.ws.cnq[b + 1] - qb0;
+  const long long block_rows = (long long)p.qbs * p.group;        // (token, head) pairs of a q-block, heads innermost
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int first = 0; first < n_qb; first += kList) {
+    // the active q-blocks among the next ones, ascending
+    int count = 0;
+    for (int i0 = first; i0 < min(first + kList, n_qb); i0 += kThreads) {
+      const int i = i0 + tid;
+      bool on = false;
+      if (i < n_qb && !(p.causal && min((i + 1) * (long long)p.qbs, (long long)q_len) - 1 + off < k0)) {
+        if (p.csr_ptr != nullptr) {
+          const long long row = (long long)hk * p.num_q_block + qb0 + i;
+          const int e1 = p.csr_ptr[row + 1], e = lower_bound_i32(p.csr_idx, p.csr_ptr[row], e1, kb);
+          on = e < e1 && p.csr_idx[e] == kb;
+        } else {
+          on = p.mask[hk * p.mask_s0 + (long long)(qb0 + i) * p.mask_s1 + (long long)kb * p.mask_s2] != 0;
+        }
+      }
+      const uint32_t bal = __ballot_sync(0xffffffffu, on);
+      __syncthreads();                           // the counts before, and the list before, have been read
+      if (lane == 0) s_count[warp] = __popc(bal);
+      __syncthreads();
+      int at = count;
+#pragma unroll
+      for (int w = 0; w < kThreads / 32; ++w) {
+        if (w < warp) at += s_count[w];
+        count += s_count[w];
+      }
+      if (on) s_list[at + __popc(bal & ((1u << lane) - 1u))] = i;
+    }
+    const long long n_tiles = (count * block_rows + kRows - 1) / kRows;
+    for (long long tile = rank; tile < n_tiles; tile += ctas) {
+      __syncthreads();                           // the list is there, and the tile before is used up
+      if (tid < kRows) {
+        const long long f = tile * kRows + tid, blk = quotient(f, block_rows);
+        long long at = -1;
+        float nl = -INFINITY;
+        int row = 0;
+        if (blk < count) {
+          const int i = s_list[blk], r = (int)(f - blk * block_rows), tok = r / p.group, h = hk * p.group + r - tok * p.group;
+          row = i * p.qbs + tok;
+          if (row < q_len) {
+            nl = P.sp.neg_lse[(((long long)(h >> P.gp_shift) * p.num_q_block + qb0 + i) * p.qbs + tok) * P.gp + (h & (P.gp - 1))];
+            if (nl != -INFINITY) at = (long long)(q_begin + row) * st.q0 + h * st.q1;
           }
         }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float nl = s_nl[rr + e];
-          const int row = i * p.qbs + (r0 + rr + e) / p.group;
-          const bool seen = nl != -INFINITY && (!p.causal || row + off >= k0 + key);
-          if (seen) tile_sum += exp2f(fmaf(s[e], P.scale_log2, nl));
-        }
+        s_at[tid] = at;
+        s_nl[tid] = nl;
+        s_pos[tid] = row + off;
       }
-      sum += tile_sum;
+      __syncthreads();
+      load(sQ, q, st.q2, [&](int r) { return s_at[r]; });
+      __syncthreads();
+      float s[4][4];
+#pragma unroll
+      for (int y = 0; y < 4; ++y)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) s[y][x] = 0.f;
+      const float *const kr = sK + tx * KS, *const qr = sQ + ty * KS;
+#pragma unroll 2
+      for (int d = 0; d < DP; d += 4) {
+        float4 a[4], c[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          a[x] = *reinterpret_cast<const float4*>(kr + 16 * x * KS + d);
+          c[x] = *reinterpret_cast<const float4*>(qr + 16 * x * KS + d);
+        }
+#pragma unroll
+        for (int y = 0; y < 4; ++y)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) s[y][x] = fmaf(a[x].x, c[y].x, fmaf(a[x].y, c[y].y, fmaf(a[x].z, c[y].z, fmaf(a[x].w, c[y].w, s[y][x]))));
+      }
+      float tile_sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const int r = ty + 16 * y;
+        const float nl = s_nl[r];
+        const int pos = s_pos[r];
+        if (nl == -INFINITY) continue;
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+          if (!p.causal || pos >= k0 + tx + 16 * x) tile_sum[x] += exp2f(fmaf(s[y][x], P.scale_log2, nl));
+      }
+#pragma unroll
+      for (int x = 0; x < 4; ++x) sum[x] += tile_sum[x];
     }
   }
-  s_sum[tid] = sum;
+#pragma unroll
+  for (int x = 0; x < 4; ++x) s_sum[ty][tx + 16 * x] = sum[x];
   __syncthreads();
-  if (tid < n_keys) P.out[(long long)(k_begin + k0 + tid) * p.nhead_k + hk] = s_sum[tid] + s_sum[tid + 64] + s_sum[tid + 128] + s_sum[tid + 192];
+  float total = 0.f;
+  if (tid < kKeys) {
+#pragma unroll
+    for (int y = 0; y < 16; ++y) total += s_sum[y][tid];
+  }
+  if (ctas > 1) {                                // the CTAs' sums, in the order of their ranks
+    __syncthreads();
+    if (tid < kKeys) s_sum[0][tid] = total;
+    ptx::cluster_sync();
+    if (rank == 0 && tid < kKeys) {
+      for (int r = 1; r < ctas; ++r) {
+        float x;
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(ptx::map_to_rank(ptx::smem_u32(&s_sum[0][tid]), (uint32_t)r)) : "memory");
+        total += x;
+      }
+    }
+    ptx::cluster_sync();                         // nobody leaves while its sums are read
+  }
+  if (rank == 0 && tid < n_keys) P.out[(long long)(k_begin + k0 + tid) * p.nhead_k + hk] = total;
 }
 
-template <typename T, int DP>
-cudaError_t launch_generic(const KeyWeightsParams& P, const hbsa_forward_args& a, cudaStream_t stream) {
-  constexpr size_t smem = sizeof(float) * (size_t)(kKeys * (DP + 4) + kRows * DP);
+template <typename T, int DP, int VEC>
+int launch_generic(const KeyWeightsParams& P, const hbsa_forward_args& a, cudaStream_t stream) {
+  constexpr size_t smem = sizeof(float) * (size_t)((kKeys + kRows) * (DP + 4));
   static SmemOptIn opt_in;
-  cudaError_t e = opt_in.once(reinterpret_cast<const void*>(key_weights_generic_kernel<T, DP>), (int)smem);
-  if (e != cudaSuccess) return e;
+  cudaError_t e = opt_in.once(reinterpret_cast<const void*>(key_weights_generic_kernel<T, DP, VEC>), (int)smem);
+  if (e != cudaSuccess) return set_last_error("hbsa_key_weights: %s", cudaGetErrorString(e)), (int)e;
   const KeyWeightsStrides st = {a.q_stride[0], a.q_stride[1], a.q_stride[2], a.k_stride[0], a.k_stride[1], a.k_stride[2]};
-  const dim3 grid((unsigned)(P.p.num_k_block * ((P.p.kbs + kKeys - 1) / kKeys)), (unsigned)P.p.nhead_k);
-  key_weights_generic_kernel<T, DP><<<grid, kThreads, smem, stream>>>(P, static_cast<const T*>(a.q), static_cast<const T*>(a.k), st);
-  return cudaGetLastError();
+  // CTAs of a cluster: as long as there are SMs for them, and two tiles for each where all q-blocks are active
+  const long long pieces = (long long)P.p.num_k_block * ((P.p.kbs + kKeys - 1) / kKeys), items = pieces * P.p.nhead_k;
+  if (pieces > INT32_MAX / 8) return set_last_error("num_k_block * k_block_size is too large"), HBSA_ERR_SHAPE;
+  const long long tiles = (long long)P.p.num_q_block * P.p.qbs * P.p.group / ((long long)kRows * P.p.batch);
+  int ctas = 1;
+  while (ctas < 8 && items * ctas < 2ll * sm100_sm_count() && tiles >= 4 * ctas) ctas *= 2;
+  cudaLaunchAttribute attr[1] = {};
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)ctas;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(pieces * ctas), (unsigned)P.p.nhead_k);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = ctas > 1 ? 1 : 0;
+  e = cudaLaunchKernelEx(&cfg, key_weights_generic_kernel<T, DP, VEC>, P, static_cast<const T*>(a.q), static_cast<const T*>(a.k), st, ctas);
+  return e == cudaSuccess ? 0 : (set_last_error("hbsa_key_weights: %s", cudaGetErrorString(e)), (int)e);
 }
 template <typename T>
-cudaError_t launch_generic_of(const KeyWeightsParams& P, const hbsa_forward_args& a, cudaStream_t stream) {
-  return a.headdim <= 64 ? launch_generic<T, 64>(P, a, stream) : a.headdim <= 128 ? launch_generic<T, 128>(P, a, stream) : launch_generic<T, 256>(P, a, stream);
+int launch_generic_of(const KeyWeightsParams& P, const hbsa_forward_args& a, cudaStream_t stream) {
+  constexpr int VEC = 16 / (int)sizeof(T);
+  bool vec = a.headdim % VEC == 0 && a.q_stride[2] == 1 && a.k_stride[2] == 1 && (uintptr_t)a.q % 16 == 0 && (uintptr_t)a.k % 16 == 0;
+  for (int i = 0; i < 2; ++i) vec = vec && a.q_stride[i] % VEC == 0 && a.k_stride[i] % VEC == 0;
+  if (a.headdim <= 64) return vec ? launch_generic<T, 64, VEC>(P, a, stream) : launch_generic<T, 64, 1>(P, a, stream);
+  if (a.headdim <= 128) return vec ? launch_generic<T, 128, VEC>(P, a, stream) : launch_generic<T, 128, 1>(P, a, stream);
+  return vec ? launch_generic<T, 256, VEC>(P, a, stream) : launch_generic<T, 256, 1>(P, a, stream);
 }
 
 size_t carve_key_weights(const hbsa_forward_args& a, char* base, KeyWeightsSpace* s) {
@@ -218,10 +319,9 @@ int hbsa_key_weights(const hbsa_key_weights_args* args, void* stream_) {
     rc = launch_key_weights_sm100(P, a, stream, &text);
     return rc != 0 ? (set_last_error("hbsa_key_weights: %s", text), rc) : 0;
   }
-  if (a.dtype == HBSA_DTYPE_BF16) e = launch_generic_of<__nv_bfloat16>(P, a, stream);
-  else if (a.dtype == HBSA_DTYPE_F16) e = launch_generic_of<__half>(P, a, stream);
-  else e = launch_generic_of<float>(P, a, stream);
-  return e == cudaSuccess ? 0 : failed(e);
+  if (a.dtype == HBSA_DTYPE_BF16) return launch_generic_of<__nv_bfloat16>(P, a, stream);
+  if (a.dtype == HBSA_DTYPE_F16) return launch_generic_of<__half>(P, a, stream);
+  return launch_generic_of<float>(P, a, stream);
 }
 
 }  // extern "C"
