@@ -99,10 +99,12 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ App
 // ------------------------------------------------------------------------------------------------------------------
 // Select: radix select of the smallest weight that stays, then one pass that writes positions in order.  The digits are 11 bits of the distance
 // from the smallest weight above zero (or, where all of those stay, from the smallest of the rest): that keeps keys that nobody has looked at
-// out of the counts, where they would meet in one bin, and spreads weights of one size over many.  A cluster of 1 to 4 CTAs per row; counts
+// out of the counts, where they would meet in one bin, and spreads weights of one size over many.  Where no more weights than threads come down
+// to the next digit (the rule after the first one), each finds its rank among them at once: 20.1 instead of 23.7 us, of 128 rows of 16384 to 32768.
+// A cluster of 1 to 4 CTAs per row; counts
 // are exchanged through distributed shared memory.  Every warp has its run of positions, in registers where they fit, as numbers that tell by
 // themselves whether the position competes; where they do not fit, they are read again for every pass.  Bound by the instructions of its
-// passes (23.7 us for 128 rows of 16384 to 32768, 35 us while every pass compared positions): memory is busy for the first one only.
+// passes (20.1 us for 128 rows of 16384 to 32768, 35 us while every pass compared positions): memory is busy for the first one only.
 constexpr int kSelectBins = 2048;
 constexpr uint32_t kGoes = 0u, kStays = 0xffffffffu, kZero = 0x80000000u;
 
@@ -126,7 +128,7 @@ __global__ void __launch_bounds__(THREADS) select_keys_kernel(const __grid_const
   __shared__ int s_hist[kSelectBins];
   __shared__ int s_more[WARPS], s_ties[WARPS], s_sum[2];
   __shared__ uint32_t s_range[4], s_prefix;
-  __shared__ int s_need;
+  __shared__ int s_need, s_here, s_found;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int row = blockIdx.x / ctas, rank = blockIdx.x - row * ctas, b = row / a.nhead_k, h = row - b * a.nhead_k;
   const int len = cut(a.lens[b], a.max_len);
@@ -151,24 +153,32 @@ __global__ void __launch_bounds__(THREADS) select_keys_kernel(const __grid_const
   bool ranged = false;
   auto place = [&](uint32_t x) { return x < low ? kGoes : x > high ? kStays : x - low + 1u; };
   auto read = [&](int from) {
+    auto inside = [&](int part) { return from + 32 * part >= lo && from + 32 * part + 256 <= min(hi, s1); };
 #pragma unroll
-    for (int part = 0; part < STEP; part += 8) {
-      const int at = from + 32 * part;
-      if (at >= lo && at + 256 <= min(hi, s1)) {
+    for (int part = 0; part < STEP; part += 8) {         // all loads first
+      const int at = from + 32 * part + lane;
+      if (inside(part)) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) u[part + e] = __float_as_uint(w[at + 32 * e + lane]);        // loads first
-#pragma unroll
-        for (int e = 0; e < 8; ++e) u[part + e] = order_of(__uint_as_float(u[part + e]));
+        for (int e = 0; e < 8; ++e) u[part + e] = __float_as_uint(w[at + 32 * e]);
       } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int i = at + 32 * e + lane;
-          u[part + e] = i >= s1 ? kGoes : i < lo || i >= hi ? kStays : order_of(w[i]);
+        for (int e = 0; e < 8; ++e) u[part + e] = at + 32 * e >= lo && at + 32 * e < min(hi, s1) ? __float_as_uint(w[at + 32 * e]) : 0u;
+      }
+    }
+#pragma unroll
+    for (int part = 0; part < STEP; part += 8) {
+#pragma unroll
+      for (int e = part; e < part + 8; ++e) u[e] = order_of(__uint_as_float(u[e]));
+      if (!inside(part)) {
+#pragma unroll
+        for (int e = part; e < part + 8; ++e) {
+          const int i = from + 32 * e + lane;
+          u[e] = i >= s1 ? kGoes : i < lo || i >= hi ? kStays : u[e];
         }
       }
       if (PER == 0 && ranged) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) u[part + e] = place(u[part + e]);
+        for (int e = part; e < part + 8; ++e) u[e] = place(u[e]);
       }
     }
   };
@@ -280,6 +290,8 @@ __global__ void __launch_bounds__(THREADS) select_keys_kernel(const __grid_const
           if (before < need && before + c[e] >= need) {
             s_prefix = prefix | (uint32_t)(top - e) << shift;
             s_need = need - before;
+            s_here = c[e];
+            s_found = 0;
             break;
           }
           before += c[e];
@@ -288,6 +300,30 @@ __global__ void __launch_bounds__(THREADS) select_keys_kernel(const __grid_const
       meet();                                            // also: all have read the counts
       prefix = s_prefix;
       need = s_need;
+      if (left > 0 && ctas == 1 && s_here <= THREADS) {  // few have come down to this digit: a thread for each, which counts those above it
+        const uint32_t from = max(prefix, 1u), size = prefix + (1u << left) - from;
+        each([&](uint32_t x, int) {
+          if (x - from < size) s_hist[atomicAdd(&s_found, 1)] = (int)x;
+        });
+        __syncthreads();
+        const int n = s_found;
+        if (tid < n) {
+          const uint32_t mine = (uint32_t)s_hist[tid];
+          int more = 0, equal = 0;
+          for (int i = 0; i < n; ++i) {
+            more += (uint32_t)s_hist[i] > mine;
+            equal += (uint32_t)s_hist[i] == mine;
+          }
+          if (more < need && more + equal >= need) {     // all threads with this number
+            s_prefix = mine;
+            s_need = need - more;
+          }
+        }
+        __syncthreads();
+        prefix = s_prefix;
+        need = s_need;
+        left = 0;
+      }
     }
     least = prefix;
     ties = need;
@@ -572,12 +608,17 @@ int hbsa_select_keys(const hbsa_select_keys_args* a, void* stream) {
   if (a->n_sink < 0 || a->n_recent < 0 || (int64_t)a->n_sink + a->n_recent > a->budget)
     return set_last_error("n_sink and n_recent must not be negative, and together not above budget"), HBSA_ERR_SHAPE;
   if ((int64_t)a->batch * a->nhead_k > INT32_MAX / 64) return set_last_error("batch * nhead_k is too large"), HBSA_ERR_SHAPE;
-  // CTAs of a row: more than one where there are SMs for them and a CTA would hold more than 8192 positions, or where one cannot hold them.
-  // 16 rows of 32768 by 1, 2, 4 and 8 CTAs: 22.8, 21.8, 17.0 and 47 us (clusters of eight full SMs do not find their places at once); 16 of
-  // 9000 by 1 and 2: 16.7 and 13.7 us; 8 of 8192 by 1 and 2: 9.9 and 13.3 us.
-  const long long rows = (long long)a->batch * a->nhead_k, places = sm100_sm_count();
-  int ctas = 1;
-  while (ctas < 4 && a->max_len > ctas * (rows * ctas * 2 <= places ? 8192 : 32768)) ctas *= 2;
+  // CTAs of a row: as many (up to 4) as bring them down to 8192 positions each where all of them have an SM, else as few as can hold the row.
+  // 16 rows of 32768 by 1, 2 and 4 CTAs: 19.7, 22.5 and 15.8 us (by 8: 47, clusters of eight full SMs do not find their places at once);
+  // 16 of 9000 by 1 and 2: 15.2 and 13.1 us; 8 of 8192 by 1 and 2: 7.4 and 13.3 us.
+  const long long rows = (long long)a->batch * a->nhead_k;
+  auto split = [&](int most) {
+    int n = 1;
+    while (n < 4 && a->max_len > n * most) n *= 2;
+    return n;
+  };
+  int ctas = split(8192);
+  if (a->max_len > ctas * 8192 || rows * ctas > sm100_sm_count()) ctas = split(32768);
   const int run = ((a->max_len + ctas - 1) / ctas + 31) & ~31;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e;
