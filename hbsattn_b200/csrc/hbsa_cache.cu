@@ -401,8 +401,7 @@ cudaError_t launch_select(const hbsa_select_keys_args& a, int ctas, cudaStream_t
 // Compact: kept positions ascend, so row j comes from row kept[j] >= j, and writing rows [c, d) touches no row that a later chunk still
 // reads.  A CTA takes one slice of the columns of one (sequence, kv-head), of K or of V, chunk by chunk: the rows of the next
 // chunk are read (their positions one chunk before), all threads meet, then the rows of this one are written.
-// Bound by latency where there are few sequences, by memory otherwise: slices of 64 bytes, so that there are enough CTAs to have 40 KB an SM
-// on their way.
+// Bound by latency where there are few sequences, by memory otherwise (8 x 4096 rows of 8 heads of 128, from 8192 to 32768: 62.4 us, 4.4 TB/s).
 struct CompactParams {
   void* cache[2];
   Rows4 rows[2];
@@ -414,7 +413,7 @@ struct CompactParams {
   int num_pages, capacity, batch, heads, units, budget;
   int lanes, slices;                     // units of a slice, slices of K and V together
 };
-constexpr int kCompactThreads = 256, kCompactUnroll = 4;
+constexpr int kCompactUnroll = 4;
 
 template <typename U> struct Chunk {
   U x[kCompactUnroll];
@@ -438,8 +437,8 @@ __device__ __forceinline__ void compact_rows(int n, int row, int rows, Next next
   }
 }
 
-template <typename U>
-__global__ void __launch_bounds__(kCompactThreads, 4) compact_kernel(const __grid_constant__ CompactParams P) {
+template <typename U, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) compact_kernel(const __grid_constant__ CompactParams P) {
   const int parts = P.slices + (P.weights != nullptr ? 1 : 0);
   const int part = blockIdx.x % parts, bh = blockIdx.x / parts, b = bh / P.heads, h = bh % P.heads;
   const int len = cut(P.lens[b], P.capacity), n = min(cut(P.kept_lens[b], P.budget), len);
@@ -451,31 +450,31 @@ __global__ void __launch_bounds__(kCompactThreads, 4) compact_kernel(const __gri
     auto next = [&](int j0) {
 #pragma unroll
       for (int e = 0; e < kCompactUnroll; ++e) {
-        const int j = j0 + e * kCompactThreads;
+        const int j = j0 + e * THREADS;
         src[e] = j < n ? kept[j] : -1;
       }
     };
     auto load = [&](Chunk<float>& c, int j0) {
 #pragma unroll
       for (int e = 0; e < kCompactUnroll; ++e) {
-        const int j = j0 + e * kCompactThreads;
+        const int j = j0 + e * THREADS;
         c.to[e] = src[e] > j && src[e] < len ? j : -1;
         if (c.to[e] >= 0) c.x[e] = w[src[e]];
       }
-      next(j0 + kCompactUnroll * kCompactThreads);
+      next(j0 + kCompactUnroll * THREADS);
     };
     auto store = [&](const Chunk<float>& c, int) {
 #pragma unroll
       for (int e = 0; e < kCompactUnroll; ++e)
         if (c.to[e] >= 0) w[c.to[e]] = c.x[e];
     };
-    compact_rows<float>(n, threadIdx.x, kCompactThreads, next, load, store);
+    compact_rows<float>(n, threadIdx.x, THREADS, next, load, store);
     __syncthreads();
-    for (int j = n + threadIdx.x; j < len; j += kCompactThreads) w[j] = 0.f;
+    for (int j = n + threadIdx.x; j < len; j += THREADS) w[j] = 0.f;
     return;
   }
   const int per = P.slices / 2, which = part / per, unit = part % per * P.lanes + threadIdx.x % P.lanes;
-  const int rows = kCompactThreads / P.lanes;
+  const int rows = THREADS / P.lanes;
   const Rows4 s = P.rows[which];
   U* const base = static_cast<U*>(P.cache[which]) + h * s.s[2] + unit * s.s[3];
   const int mine = unit < P.units ? n : 0;
@@ -663,14 +662,26 @@ int hbsa_compact_cache(const hbsa_compact_args* a, void* stream) {
   P.heads = c.nhead_k;
   P.units = c.headdim / per;
   P.budget = a->budget;
-  P.lanes = wide ? 4 : 32;
-  while (wide && P.lanes > 1 && P.lanes >= 2 * P.units) P.lanes /= 2;
-  P.slices = 2 * ((P.units + P.lanes - 1) / P.lanes);
+  // Slices of 64 bytes where that gives every SM more than one CTA, else of 32 and, for many rows, CTAs of 1024 threads, whose chunks are longer
+  // (chunk by chunk costs a round trip).  64 bytes by 256 threads against the choice, in us: 3 x 2 of 5509 rows of 256 bytes 27.2, 12.3; 1 x 8 33.2,
+  // 14.4; 2 x 8 (128 CTAs: 64 bytes by 1024 threads) 41.5, 25.6; 4 x 8 of 1000 rows of 128 bytes (32 bytes by 256 threads) 9.6, 7.1.  Where there are
+  // enough CTAs: 8 x 8 of 4096 rows 62.4, with 32 bytes 67.6, with 1024 threads 71.6.
+  auto slice = [&](int lanes) {
+    while (wide && lanes > 1 && lanes >= 2 * P.units) lanes /= 2;
+    P.lanes = lanes;
+    P.slices = 2 * ((P.units + lanes - 1) / lanes);
+    return (long long)c.batch * c.nhead_k * P.slices;
+  };
+  const int sms = sm100_sm_count();
+  const long long ctas = slice(wide ? 4 : 32);
+  const bool few = wide && ctas <= sms, many_rows = few && a->budget > 1024 && a->budget <= 1 << 30;       // (offsets behind the last row stay below 2^31)
+  if (few && (!many_rows || 2 * ctas <= sms)) slice(2);
   const unsigned grid = (unsigned)(c.batch * c.nhead_k) * (unsigned)(P.slices + (P.weights ? 1 : 0));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (wide) compact_kernel<uint4><<<grid, kCompactThreads, 0, st>>>(P);
-  else if (bytes == 2) compact_kernel<uint16_t><<<grid, kCompactThreads, 0, st>>>(P);
-  else compact_kernel<uint32_t><<<grid, kCompactThreads, 0, st>>>(P);
+  if (many_rows) compact_kernel<uint4, 1024><<<grid, 1024, 0, st>>>(P);
+  else if (wide) compact_kernel<uint4, 256><<<grid, 256, 0, st>>>(P);
+  else if (bytes == 2) compact_kernel<uint16_t, 256><<<grid, 256, 0, st>>>(P);
+  else compact_kernel<uint32_t, 256><<<grid, 256, 0, st>>>(P);
   return launched("hbsa_compact_cache");
 }
 
