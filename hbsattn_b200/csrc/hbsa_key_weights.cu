@@ -25,7 +25,44 @@ template <> __device__ __forceinline__ float to_f<float>(float x) { return x; }
 template <> __device__ __forceinline__ float to_f<__half>(__half x) { return __half2float(x); }
 template <> __device__ __forceinline__ float to_f<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
 
-// -lse log2 e of every row in the order of the tiles (-inf: nothing to add), zeros for keys outside every sample, the cleared work cursor.
+// The k-blocks by the number of rows that may see them, most first, so that the items that end a launch are short.  One CTA, 256 classes, which are
+// counted in the workspace: shared memory here would keep CTAs of the next kernel from starting beside this one (4 us of 57).
+__device__ __forceinline__ void key_weights_order(const KeyWeightsParams& P) {
+  __shared__ int s_warp[8];
+  const Problem& p = P.p;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  int* const counts = P.sp.classes;
+  counts[tid] = 0;
+  int most = 1;
+  for (int b = tid; b < p.batch; b += 256) most = max(most, p.cu_q[b + 1] - p.cu_q[b]);
+  most = __reduce_max_sync(0xffffffffu, most);
+  if (lane == 0) s_warp[warp] = most;
+  __syncthreads();
+  most = __reduce_max_sync(0xffffffffu, s_warp[lane & 7]);
+  auto class_of = [&](int kb) {
+    const int b = sample_of_block(P.ws.cnk, p.batch, kb), q_len = p.cu_q[b + 1] - p.cu_q[b], off = p.cu_k[b + 1] - p.cu_k[b] - q_len;
+    const int unseen = p.causal ? max(0, (kb - P.ws.cnk[b]) * p.kbs - off) : 0, rows = max(0, q_len - unseen);
+    return 255 - (int)(255ll * rows / most);
+  };
+  for (int kb = tid; kb < p.num_k_block; kb += 256) atomicAdd(counts + class_of(kb), 1);
+  __syncthreads();
+  const int mine = atomicAdd(counts + tid, 0);
+  int incl = mine;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, incl, d);
+    if (lane >= d) incl += y;
+  }
+  if (lane == 31) s_warp[warp] = incl;
+  __syncthreads();
+  const int before = incl - mine + __reduce_add_sync(0xffffffffu, lane < warp ? s_warp[lane & 7] : 0);
+  atomicExch(counts + tid, before);
+  __syncthreads();
+  for (int kb = tid; kb < p.num_k_block; kb += 256) P.sp.order[atomicAdd(counts + class_of(kb), 1)] = kb;
+}
+
+// -lse log2 e of every row in the order of the tiles (-inf: nothing to add), zeros for keys outside every sample, the cleared work cursor, and
+// (one CTA more) the order of the k-blocks.
 __global__ void __launch_bounds__(256) key_weights_prep_kernel(const __grid_constant__ KeyWeightsParams P, const float* __restrict__ lse) {
   const Problem& p = P.p;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -34,10 +71,14 @@ __global__ void __launch_bounds__(256) key_weights_prep_kernel(const __grid_cons
   const bool ok = P.ws.status[0] == HBSA_STATUS_OK;
   key_weights_outside(P, !ok);
   if (!ok) return;
+  if (P.sorted && blockIdx.x == gridDim.x - 1) {
+    key_weights_order(P);
+    return;
+  }
   // a warp takes 256 values of a q-block at a time, in the order of lse (rows, then heads)
   const int lane = threadIdx.x & 31, n = p.qbs * p.nhead_q, chunks = (n + 255) / 256;
   const long long todo = (long long)p.num_q_block * chunks;
-  for (long long u = blockIdx.x * 8 + (threadIdx.x >> 5); u < todo; u += gridDim.x * 8) {
+  for (long long u = blockIdx.x * 8 + (threadIdx.x >> 5); u < todo; u += (gridDim.x - P.sorted) * 8) {
     const int qb = (int)(u / chunks), first = (int)(u % chunks) * 256 + lane;
     const RowGeom g = row_geometry(p, P.ws.cnq, P.ws.cnk, P.ws.qb2b, qb);
     const float* src = lse + (long long)g.q_begin * p.nhead_q;
@@ -250,6 +291,8 @@ size_t carve_key_weights(const hbsa_forward_args& a, char* base, KeyWeightsSpace
   auto take = [&](size_t bytes) { char* r = p; p += (bytes + 255) / 256 * 256; return r; };
   s->cursor = reinterpret_cast<unsigned long long*>(take(256));
   s->neg_lse = reinterpret_cast<float*>(take((size_t)a.num_q_block * a.q_block_size * a.nhead_q * 4));
+  s->classes = reinterpret_cast<int32_t*>(take(256 * 4));
+  s->order = reinterpret_cast<int32_t*>(take(a.num_k_block <= kKwSorted ? (size_t)a.num_k_block * 4 : 0));
   return (size_t)(p - base);
 }
 
@@ -308,7 +351,13 @@ int hbsa_key_weights(const hbsa_key_weights_args* args, void* stream_) {
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(warps < most ? warps : most));
+  // Items in order, all heads of a k-block together, where some CTAs get more than one item.  Natural order (head by head) against this one, in us:
+  // causal 2 x 8192 at 10 % 86.6, 78.2; 2 x 4096 at 90 % 132, 106; not causal 2 x 1000..8192 58.1, 57.0, 33 x 20..900 56.5, 52.0, blocks of 48
+  // 54.9, 49.6; 16384 with 32 heads (134 MB of rows) 209, 199, on 8 kv-heads 258, 214.  Rows beyond the L2 are better read head by head: with 48 heads
+  // (201 MB) 296, 298.
+  const long long items = (long long)a.num_k_block * P.p.nhead_k * ((a.k_block_size + 127) / 128), streamed = (long long)a.total_q * a.nhead_q * a.headdim * 2;
+  P.sorted = impl == HBSA_IMPL_SM100 && a.num_k_block > 1 && a.num_k_block <= kKwSorted && items > 2ll * sm100_sm_count() && streamed <= 160ll << 20;
+  cfg.gridDim = dim3((unsigned)(warps < most ? warps : most) + (unsigned)P.sorted);
   cfg.blockDim = dim3(256);
   cfg.stream = stream;
   cfg.attrs = attr;

@@ -8,7 +8,10 @@ struct KeyWeightsSpace {
   unsigned long long* cursor;  // [32] word 0: next item, word 1: CTAs that have left
   float* neg_lse;              // -lse log2 e; -inf: the row adds nothing.  [nhead_q / gp][num_q_block][q_block_size][gp], blocks filled up with
                                // -inf: rows in the order of the tiles, every q-block on a 64-byte boundary whatever the samples' lengths
+  int32_t* classes;            // [256] what order is made with
+  int32_t* order;              // [num_k_block] k-blocks by the rows that may see them, most first (tensor-core kernel, where P.sorted)
 };
+constexpr int kKwSorted = 8192;              // k-blocks that are put in order, at most
 
 struct KeyWeightsParams {
   Problem p;
@@ -22,6 +25,7 @@ struct KeyWeightsParams {
   int one_box;                               // one copy brings all columns of a tile
   int m_rows, n_msub, n_cols;                // keys of an item, items per k-block, columns of S
   long long total_items;
+  int sorted;                                // items: all heads of a k-block, k-blocks in the order of sp.order; else head by head
   long long wait_budget;
   int debug_stall;
 };
