@@ -279,18 +279,11 @@ __global__ void __launch_bounds__(kGenThreads) decode_generic_kernel(const __gri
     }
   }
   __syncthreads();
+  if (tid == 0) decode_note_join(P, sh.walk);
   if (tid == 0) decode_note_status(P, sh.bad != 0 ? (int)HBSA_STATUS_CACHE_BOUNDS : (int)HBSA_STATUS_OK, P.batch - sh.bad);
 }
 
 // ------------------------------------------------------------------------------------------------------------------
-// A row of the line of tiles that several runs share: its first part is that of run c0, and there are n.
-struct DecodeParts {
-  int c0, n, slot0, lanes, lane;
-  __device__ __forceinline__ DecodeParts(const DecodeCut& cut, long long row0, int row_tiles, int lanes, int lane)
-      : c0(cut.owner(row0)), n(cut.owner(row0 + row_tiles - 1) - c0 + 1), slot0(cut.first(c0) == row0 ? 0 : 1), lanes(lanes), lane(lane) {}
-  __device__ __forceinline__ long long at(int i) const { return 2ll * ((c0 + i) * lanes + lane) + (i == 0 ? slot0 : 0); }
-};
-
 constexpr int kJoinThreads = 256;
 constexpr int kJoinMost = 1024;          // CTAs of the main kernel, at most
 
@@ -400,7 +393,7 @@ __global__ void __launch_bounds__(kJoinThreads, 4) decode_join_kernel(const __gr
   if (tid == 0) s_first = 0x7fffffff;
   pdl_wait();
   const int4 st = P.sp.cta_start[j];
-  const DecodeCut cut(*P.sp.total, P.runs);
+  const int info = P.sp.cta_join[j];
   int codes = 0;
   for (int c = tid; c < P.grid; c += kJoinThreads) codes |= 1 << P.sp.cta_status[2 * c];
   const bool gave_up = __syncthreads_or(codes & (1 << HBSA_STATUS_WAIT_LIMIT)) != 0;
@@ -427,24 +420,22 @@ __global__ void __launch_bounds__(kJoinThreads, 4) decode_join_kernel(const __gr
     return;
   }
   if (head < 0) {
-    add_weights(P, cut, st, j, (int)blockIdx.y);
+    add_weights(P, DecodeCut(*P.sp.total, P.runs), st, j, (int)blockIdx.y);
     return;
   }
-  if (st.x < 0 || st.z == 0) return;
-  const int run = j / P.lanes, hk = st.y / P.n_chunk * P.lanes + j % P.lanes, chunk = st.y % P.n_chunk;
+  if (info == 0) return;
+  const int hk = st.y / P.n_chunk * P.lanes + j % P.lanes, chunk = st.y % P.n_chunk, n = info >> 1, slot0 = info & 1;
   if (head >= min(P.chunk_heads, P.group - chunk * P.chunk_heads)) return;
-  const DecodeParts parts(cut, cut.first(run) - st.z, st.w, P.lanes, j % P.lanes);
-  if (run != parts.c0 + 1) return;
-  const int n = parts.n;
+  auto slot_of = [&](int i) { return 2ll * (j + (i - 1) * P.lanes) + (i == 0 ? slot0 : 0); };
 
   // the outputs of the first parts are on their way while the factors are made
   const int quads = P.d_pad / 4, groups = kJoinThreads / quads, quad = tid % quads, g = tid / quads;
-  auto part_of = [&](int i) { return *reinterpret_cast<const float4*>(P.sp.part_o + (parts.at(i) * kDecodeHeads + head) * P.d_pad + quad * 4); };
+  auto part_of = [&](int i) { return *reinterpret_cast<const float4*>(P.sp.part_o + (slot_of(i) * kDecodeHeads + head) * P.d_pad + quad * 4); };
   constexpr int AHEAD = 4;
   float4 early[AHEAD];
 #pragma unroll
   for (int e = 0; e < AHEAD; ++e) early[e] = g + e * groups < n ? part_of(g + e * groups) : make_float4(0.f, 0.f, 0.f, 0.f);
-  auto ml_of = [&](int i) { return *reinterpret_cast<const float2*>(P.sp.part_ml + (parts.at(i) * kDecodeHeads + head) * 2); };
+  auto ml_of = [&](int i) { return *reinterpret_cast<const float2*>(P.sp.part_ml + (slot_of(i) * kDecodeHeads + head) * 2); };
   float mx = -INFINITY;
   float2 first = make_float2(-INFINITY, 0.f);
   if (tid < n) first = ml_of(tid);
@@ -541,6 +532,7 @@ size_t carve_decode(const DecodeParams& P, char* base, DecodeSpace* s, bool own_
   s->status = reinterpret_cast<int32_t*>(take(kStatusWords * 4));
   s->cta_status = reinterpret_cast<int32_t*>(take((size_t)P.grid * 8));
   s->cta_start = reinterpret_cast<int4*>(take((size_t)P.grid * 16));
+  s->cta_join = reinterpret_cast<int32_t*>(take((size_t)P.grid * 4));
   s->total = reinterpret_cast<long long*>(take(8));
   s->pieces = reinterpret_cast<int32_t*>(take(P.mask ? rows * 4 : 0));
   s->list = reinterpret_cast<int32_t*>(take(P.mask ? rows * P.num_k_block * 4 : 0));

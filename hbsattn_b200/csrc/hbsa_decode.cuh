@@ -24,6 +24,7 @@ struct DecodeSpace {
   int32_t* status;           // [kStatusWords], written by the join kernel
   int32_t* cta_status;       // [G][2] what CTA c has to report: HBSA_STATUS_*, sequence
   int4* cta_start;           // [G] of the CTA's first row {sequence, kv-head / lanes * n_chunk + chunk, its tiles before the CTA's first, its tiles}
+  int32_t* cta_join;         // [G] 0, or, where the CTA's first row began with the CTA before: 2 * parts of the row + slot of the first one
   long long* total;          // [1] tiles of the line
   int32_t* pieces;           // [batch * nhead_k] pieces of the active blocks (mask)
   int32_t* list;             // [batch * nhead_k][num_k_block] the active blocks, ascending (mask)
@@ -91,7 +92,7 @@ struct DecodeRow {
 
 // A place on the line of tiles: the entry (a sequence, or a (sequence, kv-head) where there is a mask) and its first tile.
 struct DecodeWalk {
-  long long start, end, entry_start;
+  long long start, end, entry_start, total;
   int entry;
 };
 // Finds the place at which a CTA's run starts; all threads of the block call it.  `scratch`: shared, one word per warp.
@@ -121,8 +122,12 @@ __device__ __forceinline__ void decode_locate(const DecodeParams& P, DecodeWalk*
   if (tid == 0) {
     walk->start = start;
     walk->end = end;
+    walk->total = total;
     if (blockIdx.x == 0) *P.sp.total = total;
-    if (start == end) P.sp.cta_start[blockIdx.x] = make_int4(-1, 0, 0, 0);
+    if (start == end) {
+      P.sp.cta_start[blockIdx.x] = make_int4(-1, 0, 0, 0);
+      P.sp.cta_join[blockIdx.x] = 0;
+    }
   }
   if (start < end && start >= before && start < before + sum) {
     long long at = before;
@@ -182,9 +187,29 @@ __device__ __forceinline__ void decode_fill_empty(const DecodeParams& P, int cta
   }
 }
 
-// What every CTA of the main kernel writes down for the join: its first row.
+// A row of the line of tiles that several runs share: its first part is that of run c0, and there are n.
+struct DecodeParts {
+  int c0, n, slot0, lanes, lane;
+  __device__ __forceinline__ DecodeParts(const DecodeCut& cut, long long row0, int row_tiles, int lanes, int lane)
+      : c0(cut.owner(row0)), n(cut.owner(row0 + row_tiles - 1) - c0 + 1), slot0(cut.first(c0) == row0 ? 0 : 1), lanes(lanes), lane(lane) {}
+  __device__ __forceinline__ long long at(int i) const { return 2ll * ((c0 + i) * lanes + lane) + (i == 0 ? slot0 : 0); }
+};
+
+// What every CTA of the main kernel writes down for the join: its first row, and, once its work is under way, what there is to join.
 __device__ __forceinline__ void decode_note_start(const DecodeParams& P, const DecodeRow& r) {
   P.sp.cta_start[blockIdx.x] = make_int4(r.b, r.hk / P.lanes * P.n_chunk + r.chunk, r.tile0, r.row_tiles);
+}
+
+__device__ __forceinline__ void decode_note_join(const DecodeParams& P, const DecodeWalk& walk) {
+  if (walk.start == walk.end) return;
+  const int4 st = P.sp.cta_start[blockIdx.x];              // this thread's own
+  int info = 0;
+  if (st.z != 0) {
+    const int run = blockIdx.x / P.lanes, lane = blockIdx.x - run * P.lanes;
+    const DecodeParts parts(DecodeCut(walk.total, P.runs), walk.start - st.z, st.w, P.lanes, lane);
+    if (run == parts.c0 + 1) info = 2 * parts.n + parts.slot0;
+  }
+  P.sp.cta_join[blockIdx.x] = info;
 }
 
 __device__ __forceinline__ void decode_note_status(const DecodeParams& P, int status, int sequence) {

@@ -248,6 +248,7 @@ __global__ void __launch_bounds__(kThreads, 2) decode_f32_kernel(const __grid_co
   for (int b = blockIdx.x * kThreads + tid; b < P.batch; b += P.grid * kThreads)
     if (P.lens[b] < 0 || P.lens[b] > P.capacity) atomicMax(&sh.bad, P.batch - b);
   __syncthreads();
+  if (tid == 0) decode_note_join(P, sh.walk);
   if (tid == 0) decode_note_status(P, sh.bad != 0 ? (int)HBSA_STATUS_CACHE_BOUNDS : (int)HBSA_STATUS_OK, P.batch - sh.bad);
 }
 
