@@ -617,6 +617,13 @@ int make_decode(const hbsa_paged_attention_args* a, bool need_tensors, DecodePar
   P->runs = decode_grid(*kind, P->d_pad) / P->lanes;
   P->grid = P->runs * P->lanes;
   const bool own_lse = a->key_weights && !a->lse;
+  if (!need_tensors) {                                     // enough for whichever kernel the call gets: that depends on addresses and strides
+    const int grid = P->grid, all = sm100_sm_count() * (P->d_pad == 64 ? 4 : 2);
+    P->grid = all < kJoinMost ? all : kJoinMost;
+    *bytes = carve_decode(*P, nullptr, &P->sp, a->key_weights != nullptr);
+    P->grid = grid;
+    return 0;
+  }
   *bytes = carve_decode(*P, static_cast<char*>(a->workspace), &P->sp, own_lse);
   P->lse = own_lse ? P->sp.lse : a->lse;
   return 0;

@@ -145,7 +145,8 @@ def paged_attention(q, k_cache, v_cache, block_table, cache_lens, softmax_scale=
     ``block_mask``: bool ``(batch, nhead_k, num_k_block)`` over blocks of ``k_block_size`` positions (a multiple of 16) from the start of
     every sequence; keys of blocks that are not set are left out.  It has to cover ``max_pages * page_size`` positions.
     ``key_weights``: float32 ``(batch, nhead_k, >= max_pages * page_size)``; the attention weight of every key, summed over the q-heads of
-    its kv-head, is added to it in place (what ``select_keys`` chooses by)."""
+    its kv-head, is added to it in place (what ``select_keys`` chooses by).  The call then holds every score for its duration: 4 bytes per
+    q-head and position of ``batch * max_pages * page_size``."""
     result = _host.paged(q, k_cache, v_cache, block_table, cache_lens, softmax_scale, block_mask, k_block_size, key_weights, bool(return_lse))
     if result is not None:
         return result

@@ -329,7 +329,8 @@ int hbsa_append_to_cache(const hbsa_append_args* args, void* stream);
  *   key_weights   NULL, or float32 [batch, nhead_k, >= max_pages * page_size], strides in elements (unit along the last):
  *                 receives, added to what is there, the attention weight of every key summed over the q-heads of its kv-head
  * The tensor-core kernel takes bf16/fp16, headdim a multiple of 8 from 16 to 256 with unit stride, 16-byte aligned rows, a page
- * size that is a multiple of 16 and softmax_scale > 0; a CUDA-core kernel takes the rest.  Should a wait inside the former
+ * size that is a multiple of 16 and softmax_scale > 0; CUDA-core kernels take the rest, one of them fp32 of 16-byte aligned
+ * rows and a page size that is a multiple of 8.  Should a wait inside the tensor-core kernel
  * run out, the status word says HBSA_STATUS_WAIT_LIMIT, o and lse are NaN, and key_weights are left as they were.
  */
 typedef struct hbsa_paged_attention_args {
@@ -354,7 +355,8 @@ typedef struct hbsa_paged_attention_args {
   size_t workspace_bytes;
 } hbsa_paged_attention_args;
 
-/* Depends on the sizes, the dtype, and on which of block_mask and key_weights are given; asks the current device for its number of SMs. */
+/* Depends on the sizes, the dtype, and on which of block_mask and key_weights are given; asks the current device for its number of SMs.
+ * With key_weights it holds the scores: 4 bytes per q-head and position of batch * max_pages * page_size. */
 size_t hbsa_paged_attention_workspace_bytes(const hbsa_paged_attention_args* args);
 int hbsa_paged_attention(const hbsa_paged_attention_args* args, void* stream);
 

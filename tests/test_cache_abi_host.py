@@ -119,3 +119,24 @@ def test_operators_refuse_cpu_tensors():
                  lambda: hb.compact_cache(cache, cache, table, lens, table[None], lens)):
         with pytest.raises(RuntimeError, match="CUDA"):
             call()
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_workspace_does_not_depend_on_addresses_and_strides(d, dtype):
+    """A size that was asked for without tensors is enough for whichever kernel the tensors lead to."""
+
+    from hbsattn_b200 import _lib
+    lib = _lib.load()
+    a = _lib.PagedAttentionArgs()
+    a.struct_bytes = ctypes.sizeof(a)
+    a.cache.num_pages, a.cache.page_size, a.cache.nhead_k, a.cache.headdim = 10, 16, 2, d
+    a.cache.batch, a.cache.max_pages, a.cache.dtype, a.nhead_q, a.use_default_scale = 3, 4, dtype, 8, 1
+    asked = lib.hbsa_paged_attention_workspace_bytes(ctypes.byref(a))
+    a.cache.k = a.cache.v = a.q = a.o = 1 << 20
+    for strides in ((16 * 2 * d, 2 * d, d, 1), (16 * 2 * (d + 1), 2 * (d + 1), d + 1, 1)):
+        for i in range(4):
+            a.cache.k_stride[i] = a.cache.v_stride[i] = strides[i]
+        for i in range(3):
+            a.q_stride[i] = a.o_stride[i] = strides[i + 1]
+        assert lib.hbsa_paged_attention_workspace_bytes(ctypes.byref(a)) == asked > 0
