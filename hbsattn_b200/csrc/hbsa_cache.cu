@@ -63,7 +63,7 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ App
   for (long long tok = lo + (long long)blockIdx.x * 8 + (threadIdx.x >> 5); tok < hi; tok += (gridDim.x - 1) * 8ll) {
     const int b = sample_of_block(P.cu, P.batch, (int)tok);
     const long long pos = (long long)cut(P.lens[b], P.capacity) + (tok - P.cu[b]);
-    if (pos >= P.capacity) continue;
+    if (pos >= P.capacity) continue;                       // (never negative: cu[b] <= tok whatever cu holds)
     int slot;
     const int page = P.table[b * P.table_stride + P.page.split((int)pos, slot)];
     if (page < 0 || page >= P.num_pages) continue;
@@ -367,7 +367,8 @@ __global__ void __launch_bounds__(THREADS) select_keys_kernel(const __grid_const
     const uint32_t from = all ? least : least + 1u;      // (least is kStays only where all of them do)
     each([&](uint32_t x, int at) {
       const uint32_t bal = __ballot_sync(0xffffffffu, x >= from);
-      if (x >= from) kept[out + __popc(bal & below)] = at + lane;
+      const int to = out + __popc(bal & below);
+      if (x >= from && (PER > 0 || to < a.budget)) kept[to] = at + lane;       // (weights that somebody changes between two reads)
       out += __popc(bal);
     });
   } else {
@@ -375,7 +376,8 @@ __global__ void __launch_bounds__(THREADS) select_keys_kernel(const __grid_const
       const uint32_t tied = __ballot_sync(0xffffffffu, x == least);
       const bool stays = x > least || (x == least && tie + __popc(tied & below) < ties);
       const uint32_t bal = __ballot_sync(0xffffffffu, stays);
-      if (stays) kept[out + __popc(bal & below)] = at + lane;
+      const int to = out + __popc(bal & below);
+      if (stays && (PER > 0 || to < a.budget)) kept[to] = at + lane;
       out += __popc(bal);
       tie += __popc(tied);
     });
