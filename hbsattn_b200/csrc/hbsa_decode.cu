@@ -613,7 +613,7 @@ int make_decode(const hbsa_paged_attention_args* a, bool need_tensors, DecodePar
   if (P->mask) P->unit = gcd(P->unit, P->kbs);
   P->pieces_per_block = P->mask ? P->kbs / P->unit : 0;
   P->one_box = P->headdim % 64 == 0;
-  P->lanes = P->mask || P->nhead_k % 2 ? 1 : P->nhead_k % 4 ? 2 : 4;
+  P->lanes = P->mask || P->nhead_k % 2 ? 1 : 2;
   P->runs = decode_grid(*kind, P->d_pad) / P->lanes;
   P->grid = P->runs * P->lanes;
   const bool own_lse = a->key_weights && !a->lse;

@@ -5,10 +5,12 @@
 // block mask tile i holds positions 64 i .. 64 i + 63, with one the tile is strung together from pieces of `unit` positions of the
 // active blocks.  The tiles of all rows stand in one line (sequence, kv-head, chunk, tile), which is cut into runs of the same
 // length, up to one tile: every CTA reads the same number of keys, whatever the lengths are, and at most its first and its
-// last row are shared with neighbours.  Without a mask `lanes` (1, 2 or 4) neighbouring kv-heads are worked on side by side: the line holds
-// every lanes-th kv-head, and the CTAs lanes * c .. take run c of it, one kv-head each, so that what lies together in memory is
-// read at the same time (16 x 24576 keys, 8 heads of 64 inside the slots: 160 us with one lane).  Those leave (maximum, sum, unnormalised output) in two slots of the CTA's own, which the
+// last row are shared with neighbours.  Those leave (maximum, sum, unnormalised output) in two slots of the CTA's own, which the
 // join kernel puts together in the order of the CTAs, so that results do not depend on timing.
+// Without a mask two neighbouring kv-heads (`lanes`; one where their number is odd) are worked on side by side: the line holds
+// every other kv-head, and the CTAs lanes * c .. take run c of it, one kv-head each, so that what lies together in memory is read
+// at the same time (16 x 24576 keys, 8 heads inside the slots: of 64 157 us with one lane, 133 with two and with four; of 128
+// 130 us with any).
 #pragma once
 #include "hbsa_common.cuh"
 
