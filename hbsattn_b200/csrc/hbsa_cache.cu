@@ -620,6 +620,8 @@ int hbsa_select_keys(const hbsa_select_keys_args* a, void* stream) {
   };
   int ctas = split(8192);
   if (a->max_len > ctas * 8192 || rows * ctas > sm100_sm_count()) ctas = split(32768);
+  // Threads and positions a thread: 10 rows of 1000 by 256 and by 1024 threads 4.7 and 6.8 us, 128 rows 8.2 and 24.9; 128 rows of up to 32768 in
+  // registers 20.4, read again for every pass 30.4.
   const int run = ((a->max_len + ctas - 1) / ctas + 31) & ~31;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e;
