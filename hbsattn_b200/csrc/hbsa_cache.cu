@@ -10,7 +10,8 @@ namespace {
 struct Rows4 { long long s[4]; };        // strides in units: page, slot, head, unit
 
 // ------------------------------------------------------------------------------------------------------------------
-// Append: one warp per new token, K and V together.  The last block writes the new lengths and the status.
+// Append: one warp per new token, K and V together, four units of each on their way a lane.  The last block writes the new lengths and the status.
+// One token of 16 sequences, 8 heads of 64: 2.6 us (a launch); 8 x 1024..16384 tokens, 8 heads of 128: 78 us (480 MB, 6.2 TB/s).
 struct AppendParams {
   const void *k, *v;
   void *k_cache, *v_cache;
