@@ -18,7 +18,7 @@
 // At the end of a row the warps' parts are put together through shared memory, up to 128 columns at a time.
 // P enters P V in the type of V, as in the prompt's kernels: at most 2^-8 (bf16) or 2^-11 (fp16) of a term, what the rounding of the output costs too (bf16
 // over 16384..32768 keys: 1.8e-3 of the output against 64 bits, 1.6e-3 with P in fp32).  Scores, statistics and sums are fp32.
-// Measured: 16 x 16384..32768 keys, 8 heads of 64, groups of 8: 123 us, of which 102 are the stream (745 MB, 7.3 TB/s), 6 the way to the first tile, 6
+// Measured: 16 x 16384..32768 keys, 8 heads of 64, groups of 8: 125 us, of which 102 are the stream (745 MB, 7.3 TB/s), 6 the way to the first tile, 6
 // the join; 8 x 16384..65536 keys, 30 % of the blocks, 8 heads of 128: 98 us (527 MB).  A call without work to speak of: 10.5 us.
 // Positions behind the length share the last tile with others and may hold anything: their scores are set to -inf, and their
 // rows of V to zero in shared memory (0 x NaN would come out of the product otherwise).
