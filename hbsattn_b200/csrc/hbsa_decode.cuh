@@ -31,7 +31,7 @@ struct DecodeSpace {
   int32_t* pieces;           // [batch * nhead_k] pieces of the active blocks (mask)
   int32_t* list;             // [batch * nhead_k][num_k_block] the active blocks, ascending (mask)
   float* lse;                // [batch, nhead_q] (weights, where the caller wants no lse)
-  float* part_ml;            // [2 G][kDecodeHeads][2] maximum (log2 domain) and sum
+  float* part_ml;            // [2 G][kDecodeHeads][2] what the part is relative to (log2 domain: its maximum, in fp16 14 less) and its sum
   float* part_o;             // [2 G][kDecodeHeads][d_pad]
   float* scores;             // [batch, nhead_q, capacity] scaled scores in the log2 domain (weights)
 };

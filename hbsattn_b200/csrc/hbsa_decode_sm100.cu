@@ -17,7 +17,11 @@
 //               of O's columns each (the scores are made twice), and Q is read from shared memory for every product.
 // At the end of a row the warps' parts are put together through shared memory, up to 128 columns at a time.
 // P enters P V in the type of V, as in the prompt's kernels: at most 2^-8 (bf16) or 2^-11 (fp16) of a term, what the rounding of the output costs too (bf16
-// over 16384..32768 keys: 1.8e-3 of the output against 64 bits, 1.6e-3 with P in fp32).  Scores, statistics and sums are fp32.
+// over 16384..32768 keys: 1.8e-3 of the output against 64 bits, 1.6e-3 with P in fp32).  In fp16 that holds for normal numbers only, so P is formed
+// against the maximum less 14 there: the largest is 2^14 (of 2^16 that fp16 has), and rounding is by 2^-11 of a term down to 2^-28 of the largest, by at most
+// 2^-39 of the largest below.  Against the maximum itself everything below 2^-25 was lost (equal keys 19 nats below sinks that every
+// warp meets: all of their share; now within 2^-10 of it, in the same time).  The factor is in O, the sums and the maxima that are handed on, and
+// leaves with the division.  Scores, statistics and sums are fp32.
 // Measured: 16 x 16384..32768 keys, 8 heads of 64, groups of 8: 125 us, of which 102 are the stream (745 MB, 7.3 TB/s), 6 the way to the first tile, 6
 // the join; 8 x 16384..65536 keys, 30 % of the blocks, 8 heads of 128: 98 us (527 MB).  A call without work to speak of: 10.5 us.
 // Positions behind the length share the last tile with others and may hold anything: their scores are set to -inf, and their
@@ -104,6 +108,8 @@ decode_sm100_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
   constexpr uint32_t HALF = (uint32_t)Shape<D>::kKeys * D * 2u, STAGE = 2 * HALF;      // bytes of K or V, and of both
   constexpr bool HALVES = Shape<D>::kHalves;
   constexpr int COLUMNS = Shape<D>::kColumns;
+  // P = 2^(score - reference(maximum)).  Beyond 2^24 subtracting 14 may subtract 16, and 2^16 is no fp16 number.
+  auto reference = [](float m) { return BF16 || fabsf(m) >= 16777216.f ? m : m - 14.f; };
   using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
   extern __shared__ __align__(1024) uint8_t base[];  // 1024-byte aligned tiles for the 128-byte swizzle
   const uint32_t ring = smem_u32(base);
@@ -366,7 +372,8 @@ decode_sm100_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
               x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 1));
               x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 2));
               x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 2));
-              const float a0 = x0 == -INFINITY ? 1.f : ex2_approx(m0 - x0), a1 = x1 == -INFINITY ? 1.f : ex2_approx(m1 - x1);
+              // (the references' difference is not the maxima's: subtracting 14 may round)
+              const float a0 = x0 == -INFINITY ? 1.f : ex2_approx(reference(m0) - reference(x0)), a1 = x1 == -INFINITY ? 1.f : ex2_approx(reference(m1) - reference(x1));
               l0 *= a0;
               l1 *= a1;
 #pragma unroll
@@ -379,7 +386,7 @@ decode_sm100_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
               m0 = x0;
               m1 = x1;
             }
-            const float r0 = m0 == -INFINITY ? 0.f : m0, r1 = m1 == -INFINITY ? 0.f : m1;
+            const float r0 = m0 == -INFINITY ? 0.f : reference(m0), r1 = m1 == -INFINITY ? 0.f : reference(m1);
             uint32_t p[UNITS][4];
 #pragma unroll
             for (int j = 0; j < 2 * UNITS; ++j) {
@@ -443,8 +450,8 @@ decode_sm100_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
       for (int c0 = 0; c0 < COLUMNS; c0 += width) {
         if (!(ok = part_writable())) break;
         if (t4 == 0) {
-          *reinterpret_cast<float2*>(ctl->ml[warp][g]) = make_float2(m0, l0);
-          *reinterpret_cast<float2*>(ctl->ml[warp][g + 8]) = make_float2(m1, l1);
+          *reinterpret_cast<float2*>(ctl->ml[warp][g]) = make_float2(reference(m0), l0);
+          *reinterpret_cast<float2*>(ctl->ml[warp][g + 8]) = make_float2(reference(m1), l1);
         }
 #pragma unroll
         for (int i = 0; i < COLUMNS / 8; ++i) {
