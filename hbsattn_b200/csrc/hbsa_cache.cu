@@ -35,9 +35,9 @@ __device__ __forceinline__ void append_status(const AppendParams& P) {
   int per = 1;                           // threads of a sequence
   while (per < 32 && per * 2 * P.batch <= threads) per *= 2;
   for (int b = tid / per; b < P.batch; b += threads / per) {
-    const int raw = P.lens[b], len = cut(raw, P.capacity), n = max(0, P.cu[b + 1] - P.cu[b]);
-    const int end = (int)min((long long)len + n, (long long)P.capacity);
-    bool bad = raw != len || (long long)len + n > P.capacity;
+    const int raw = P.lens[b], len = cut(raw, P.capacity), c0 = P.cu[b], c1 = P.cu[b + 1], n = max(0, cut(c1, P.total) - cut(c0, P.total));
+    const int end = (int)min((long long)len + n, (long long)P.capacity);       // (only rows that are there count: what is read later has been written)
+    bool bad = raw != len || (long long)len + n > P.capacity || c0 < 0 || c1 < c0 || c1 > P.total;
     if (end > len)
       for (int i = P.page.quotient(len) + tid % per; i <= P.page.quotient(end - 1); i += per) {
         const int page = P.table[b * P.table_stride + i];
@@ -63,7 +63,7 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ App
   const int lo = max(0, P.cu[0]), hi = min(P.total, P.cu[P.batch]);
   for (long long tok = lo + (long long)blockIdx.x * 8 + (threadIdx.x >> 5); tok < hi; tok += (gridDim.x - 1) * 8ll) {
     const int b = sample_of_block(P.cu, P.batch, (int)tok);
-    const long long pos = (long long)cut(P.lens[b], P.capacity) + (tok - P.cu[b]);
+    const long long pos = (long long)cut(P.lens[b], P.capacity) + (tok - max(0, P.cu[b]));
     if (pos >= P.capacity) continue;                       // (never negative: cu[b] <= tok whatever cu holds)
     int slot;
     const int page = P.table[b * P.table_stride + P.page.split((int)pos, slot)];

@@ -105,7 +105,8 @@ def _run(name, args, device):
 def append_to_cache(k, v, cu_seqlens, k_cache, v_cache, block_table, cache_lens):
     """Writes new tokens behind those that every sequence holds already: row ``cu_seqlens[b] + i`` of ``k`` and ``v`` (packed
     ``(total, nhead_k, headdim)``, any strides) goes to position ``cache_lens[b] + i`` of sequence ``b``.  Rows outside every sequence are
-    not read.  Returns the new lengths, int32 ``[batch]``; ``cache_lens`` itself is left as it is."""
+    not read; a ``cu_seqlens`` that leaves ``[0, total]`` is cut to it, and ``last_status()`` says ``HBSA_STATUS_CACHE_BOUNDS``.  Returns
+    the new lengths, int32 ``[batch]``; ``cache_lens`` itself is left as it is."""
     new_lens = _host.append(k, v, cu_seqlens, k_cache, v_cache, block_table, cache_lens)     # None: what it does not take goes on here
     if new_lens is not None:
         return new_lens

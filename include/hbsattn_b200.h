@@ -50,8 +50,9 @@ enum {
   HBSA_STATUS_BLOCK_COUNT_MISMATCH = 1, /* num_q_block/num_k_block differ from what cu_seqlens imply;
                                            no attention is computed and `o` is filled with zeros  */
   HBSA_STATUS_WAIT_LIMIT = 2,           /* a bounded wait inside the attention kernel ran out       */
-  HBSA_STATUS_CACHE_BOUNDS = 3          /* a paged cache: a length is outside [0, max_pages * page_size] or a page index outside
-                                           [0, num_pages); what lies there is left out. Word 1: the first such sequence   */
+  HBSA_STATUS_CACHE_BOUNDS = 3          /* a paged cache: a length is outside [0, max_pages * page_size], a page index outside
+                                           [0, num_pages), or (append) the sequence's rows outside [0, total); what lies there is
+                                           left out. Word 1: the first such sequence                                      */
 };
 
 /* Library / ABI version (HBSA_ABI_VERSION of the build). */
@@ -300,8 +301,9 @@ typedef struct hbsa_cache {
 /*
  * Writes new tokens behind those that a sequence holds already: token i of sequence b, row cu_seqlens[b] + i of k and v
  * (packed [total, nhead_k, headdim], strides in elements), goes to position cache.lens[b] + i.  Rows of k and v outside
- * every sequence are not read, positions outside the cache are not written.
- *   new_lens   int32 [batch]: lens[b] plus the number of its new tokens, cut to the cache's capacity
+ * every sequence are not read, positions outside the cache are not written.  cu_seqlens has to ascend within [0, total]; it is
+ * cut to that, and HBSA_STATUS_CACHE_BOUNDS says so.
+ *   new_lens   int32 [batch]: lens[b] plus the number of its rows, cut to the cache's capacity
  *   status     16 int32 words (device) that hbsa_read_status reads
  */
 typedef struct hbsa_append_args {
