@@ -73,7 +73,7 @@ struct DecodeGenericShared {
   long long k_at[kDecodeTile], v_at[kDecodeTile];      // element offset of every key's row; < 0: no such key
   int pos[kDecodeTile];                                // position in the sequence, or -1
   float m[kDecodeHeads], l[kDecodeHeads], alpha[kDecodeHeads];
-  int bad;                                             // 1 + a sequence with a length or a page out of range
+  int bad;                                             // the first sequence with a length or a page out of range, from the end (0: none)
 };
 
 template <int DP> constexpr size_t generic_smem() {

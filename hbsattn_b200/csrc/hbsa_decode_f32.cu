@@ -23,7 +23,7 @@ struct F32Shared {
   DecodeWalk walk;
   long long scratch[kWarps];
   float2 ml[kWarps][8];
-  int bad;                                             // 1 + a sequence with a length or a page out of range, from the end
+  int bad;                                             // the first sequence with a length or a page out of range, from the end (0: none)
 };
 
 template <int DP, int HEADS>

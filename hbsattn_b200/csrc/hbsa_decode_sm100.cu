@@ -64,7 +64,7 @@ template <int D> struct __align__(16) DecodeControl {
   long long scratch[16];
   DecodeRow row[kRowSlots];
   float ml[kConsumers][16][2];
-  int abort_flag, bad;
+  int abort_flag, bad;   // bad: the first sequence with a length or a page out of range, from the end (0: none)
 };
 
 constexpr uint32_t kPartBytes = kConsumers * 16 * 64 * 4;
@@ -183,7 +183,7 @@ decode_sm100_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
       while (first < end && ok) {
         look_up(first + 32 + lane, next_pos, next_page);
         const bool bad = pos >= 0 && (page < 0 || page >= P.num_pages);
-        if (__any_sync(0xffffffffu, bad) && lane == 0) ctl->bad = 1 + r.b;
+        if (__any_sync(0xffffffffu, bad) && lane == 0) atomicMax(&ctl->bad, P.batch - r.b);
         const int n_keys = pos < 0 || bad ? 0 : min(P.unit, r.len - pos), n_hidden = bad ? min(P.unit, r.len - pos) : 0;
         const int slot = pos < 0 ? 0 : pos % P.page;
         const uint32_t there = __ballot_sync(0xffffffffu, n_keys > 0);
@@ -511,11 +511,11 @@ decode_sm100_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
   __syncthreads();
   decode_fill_empty<T>(P, blockIdx.x, P.grid);
   for (int b = blockIdx.x * kThreads + tid; b < P.batch; b += P.grid * kThreads)
-    if (P.lens[b] < 0 || P.lens[b] > P.capacity) ctl->bad = 1 + b;
+    if (P.lens[b] < 0 || P.lens[b] > P.capacity) atomicMax(&ctl->bad, P.batch - b);
   __syncthreads();
   if (tid == 0) {
     const int bad = ctl->bad;
-    decode_note_status(P, ctl->abort_flag != 0 ? (int)HBSA_STATUS_WAIT_LIMIT : bad != 0 ? (int)HBSA_STATUS_CACHE_BOUNDS : (int)HBSA_STATUS_OK, bad - 1);
+    decode_note_status(P, ctl->abort_flag != 0 ? (int)HBSA_STATUS_WAIT_LIMIT : bad != 0 ? (int)HBSA_STATUS_CACHE_BOUNDS : (int)HBSA_STATUS_OK, P.batch - bad);
   }
 }
 
