@@ -287,6 +287,12 @@ int launch_generic_of(const KeyWeightsParams& P, const hbsa_forward_args& a, cud
   return vec ? launch_generic<T, 256, VEC>(P, a, stream) : launch_generic<T, 256, 1>(P, a, stream);
 }
 
+// A block that holds every packed row there is: larger ones are no different, as every sample is one block of them, and cost workspace.
+int32_t block_within(int32_t block, int32_t total) {
+  const long long all = ((long long)total + 127) / 128 * 128;
+  return total > 0 && block % 16 == 0 && block > all ? (int32_t)all : block;
+}
+
 size_t carve_key_weights(const hbsa_forward_args& a, char* base, KeyWeightsSpace* s) {
   char* p = base;
   auto take = [&](size_t bytes) { char* r = p; p += (bytes + 255) / 256 * 256; return r; };
@@ -306,7 +312,9 @@ extern "C" {
 size_t hbsa_key_weights_workspace_bytes(const hbsa_key_weights_args* args) {
   if (!args || args->struct_bytes != sizeof(*args) || args->fwd.num_q_block <= 0 || args->fwd.q_block_size <= 0 || args->fwd.nhead_q <= 0) return 0;
   hbsa::KeyWeightsSpace s;
-  return hbsa::carve_key_weights(args->fwd, nullptr, &s);
+  hbsa_forward_args a = args->fwd;
+  a.q_block_size = hbsa::block_within(a.q_block_size, a.total_q);
+  return hbsa::carve_key_weights(a, nullptr, &s);
 }
 
 int hbsa_key_weights(const hbsa_key_weights_args* args, void* stream_) {
@@ -316,6 +324,8 @@ int hbsa_key_weights(const hbsa_key_weights_args* args, void* stream_) {
   KeyWeightsParams P;
   memset(&P, 0, sizeof(P));
   hbsa_forward_args a = args->fwd;
+  a.q_block_size = block_within(a.q_block_size, a.total_q);
+  a.k_block_size = block_within(a.k_block_size, a.total_k);
   a.v = a.k;                                   // not used: the checks of a forward apply to what is there
   a.o = const_cast<void*>(a.q);
   for (int i = 0; i < 3; ++i) {
@@ -324,6 +334,7 @@ int hbsa_key_weights(const hbsa_key_weights_args* args, void* stream_) {
   }
   int rc = make_problem(&a, true, &P.p);
   if (rc != 0) return rc;
+  if ((int64_t)a.q_block_size * a.nhead_q > INT32_MAX - 512) return set_last_error("q-blocks of more than 2^31 rows (tokens x q-heads) are not supported"), HBSA_ERR_SHAPE;
   if (!a.lse || !args->weights || !args->partial_workspace) return set_last_error("lse, weights and partial_workspace must not be NULL"), HBSA_ERR_NULL;
   if (args->partial_workspace_bytes < carve_key_weights(a, static_cast<char*>(args->partial_workspace), &P.sp))
     return set_last_error("partial_workspace is smaller than hbsa_key_weights_workspace_bytes()"), HBSA_ERR_WORKSPACE;
