@@ -82,10 +82,11 @@ __global__ void __launch_bounds__(256) key_weights_prep_kernel(const __grid_cons
     const int qb = (int)(u / chunks), first = (int)(u % chunks) * 256 + lane;
     const RowGeom g = row_geometry(p, P.ws.cnq, P.ws.cnk, P.ws.qb2b, qb);
     const float* src = lse + (long long)g.q_begin * p.nhead_q;
-    const int there = (g.q_end - g.q_begin) * p.nhead_q;
+    // (rows that cu_q puts outside the tensors add nothing and are not read)
+    const int missing = max(0, min(-g.q_begin, p.qbs)) * p.nhead_q, there = max(0, min(g.q_end, P.total_q) - g.q_begin) * p.nhead_q;
     float x[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = first + 32 * e < there ? src[first + 32 * e] : -INFINITY;
+    for (int e = 0; e < 8; ++e) x[e] = first + 32 * e >= missing && first + 32 * e < there ? src[first + 32 * e] : -INFINITY;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const int i = first + 32 * e, tok = i / p.nhead_q, h = i - tok * p.nhead_q;
@@ -137,7 +138,7 @@ __global__ void __launch_bounds__(kThreads, DP == 256 ? 1 : 2) key_weights_gener
       }
     }
   };
-  load(sK, k, st.k2, [&](int r) { return r < n_keys ? (long long)(k_begin + k0 + r) * st.k0 + hk * st.k1 : -1ll; });
+  load(sK, k, st.k2, [&](int r) { return r < n_keys && key_is_there(P, k_begin + k0 + r) ? (long long)(k_begin + k0 + r) * st.k0 + hk * st.k1 : -1ll; });
   const int qb0 = P.ws.cnq[b], n_qb = P.ws.cnq[b + 1] - qb0;
   const long long block_rows = (long long)p.qbs * p.group;        // (token, head) pairs of a q-block, heads innermost
   float sum[4] = {0.f, 0.f, 0.f, 0.f};
@@ -246,7 +247,7 @@ __global__ void __launch_bounds__(kThreads, DP == 256 ? 1 : 2) key_weights_gener
     }
     ptx::cluster_sync();                         // nobody leaves while its sums are read
   }
-  if (rank == 0 && tid < n_keys) P.out[(long long)(k_begin + k0 + tid) * p.nhead_k + hk] = total;
+  if (rank == 0 && tid < n_keys && key_is_there(P, k_begin + k0 + tid)) P.out[(long long)(k_begin + k0 + tid) * p.nhead_k + hk] = total;
 }
 
 template <typename T, int DP, int VEC>

@@ -30,6 +30,9 @@ struct KeyWeightsParams {
   int debug_stall;
 };
 
+// Keys that cu_k puts outside the tensors are neither read nor written.
+__device__ __forceinline__ bool key_is_there(const KeyWeightsParams& P, int row) { return (unsigned)row < (unsigned)P.total_k; }
+
 // Keys outside every sample get zeros, and with a block count mismatch all keys do.  All threads of the grid.
 __device__ __forceinline__ void key_weights_outside(const KeyWeightsParams& P, bool all) {
   const int lo = all ? 0 : max(0, min(P.p.cu_k[0], P.total_k)), hi = all ? 0 : max(lo, min(P.p.cu_k[P.p.batch], P.total_k));

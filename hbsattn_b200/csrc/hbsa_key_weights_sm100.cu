@@ -250,7 +250,8 @@ key_weights_sm100_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_
         for (int d = 16; d > 0; d >>= 1) n += __shfl_xor_sync(0xffffffffu, n, d);
         n_tiles = (n * P.n_head_sub + per_tile - 1) >> (TILE_SHIFT - P.piece_shift);
         if (n_tiles == 0) {
-          for (int j = lane; j < keys; j += 32) P.out[(long long)(k_begin + k0 + j) * p.nhead_k + hk] = 0.f;
+          for (int j = lane; j < keys; j += 32)
+            if (key_is_there(P, k_begin + k0 + j)) P.out[(long long)(k_begin + k0 + j) * p.nhead_k + hk] = 0.f;
           continue;
         }
       }
@@ -517,7 +518,7 @@ key_weights_sm100_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_
       }
       if (!ok) break;
       if (KEYS) {
-        if (row < keys) P.out[(long long)(row0 + row) * p.nhead_k + head] = total;
+        if (row < keys && key_is_there(P, row0 + row)) P.out[(long long)(row0 + row) * p.nhead_k + head] = total;
       } else {
         // the sums of the warp's 32 rows, then those of the four warps (the slots see to it that the sums of the item before the last
         // one have been read)
@@ -542,8 +543,8 @@ key_weights_sm100_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_
             sum.y += *(volatile float*)&ctl->sums[I & 1][w][2 * lane + 1];
           }
           float* const out = P.out + (long long)(row0 + 2 * lane) * p.nhead_k + head;
-          if (2 * lane < keys) out[0] = sum.x;
-          if (2 * lane + 1 < keys) out[p.nhead_k] = sum.y;
+          if (2 * lane < keys && key_is_there(P, row0 + 2 * lane)) out[0] = sum.x;
+          if (2 * lane + 1 < keys && key_is_there(P, row0 + 2 * lane + 1)) out[p.nhead_k] = sum.y;
         }
       }
       __syncwarp();

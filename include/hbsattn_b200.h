@@ -366,7 +366,8 @@ int hbsa_paged_attention(const hbsa_paged_attention_args* args, void* stream);
  * The attention weight that the queries of a forward call give to every key, summed over the rows that see it and over the
  * q-heads of its kv-head: weights[j, hk] = sum exp(scale q.k_j - lse), float32 [total_k, nhead_k] (contiguous).
  * `fwd` describes the call: q, k, the forward's lse (required), mask, sizes, workspace (the schedule is rebuilt in it); v and
- * o are not used.  Keys outside every sample get zeros.  Rows whose lse is -inf add nothing.  The tcgen05 kernel runs what
+ * o are not used.  Keys outside every sample get zeros.  Rows whose lse is -inf add nothing, nor do rows that cu_q_seqlens puts outside
+ * [0, total_q); keys that cu_k_seqlens puts outside [0, total_k) are neither read nor written.  The tcgen05 kernel runs what
  * the forward's takes; should a wait inside it run out, the status word says HBSA_STATUS_WAIT_LIMIT and the weights are NaN.
  * partial_workspace: >= hbsa_key_weights_workspace_bytes(...) bytes, 256-byte aligned.
  */

@@ -1,4 +1,4 @@
-"""Key weights at the ends of what the arguments allow: blocks larger than everything that is packed."""
+"""Key weights at the ends of what the arguments allow, and beyond: blocks larger than everything that is packed, samples that reach beyond the tensors."""
 import pytest
 import torch
 
@@ -47,3 +47,30 @@ def test_the_size_of_the_workspace_goes_by_the_rows():
     assert len(set(sizes)) == 1 and sizes[0] < 1 << 20
     f.q_block_size, f.total_q = 1024, 0                   # not known yet: enough for any
     assert lib.hbsa_key_weights_workspace_bytes(ctypes.byref(a)) >= 3 * 1024 * 16 * 4
+
+
+@pytest.mark.parametrize("family", ["auto", "generic"])
+@pytest.mark.parametrize("kbs", [64, 128])
+@pytest.mark.parametrize("hq,hk,d,causal,dtype", [(8, 2, 64, True, torch.bfloat16), (3, 3, 128, False, torch.float16), (4, 1, 32, True, torch.float32)])
+def test_samples_that_reach_beyond_the_tensors(hq, hk, d, causal, dtype, kbs, family):
+    """Rows and keys before the first and behind the last one that is there: not read, not written, and without weight."""
+    import hbsattn_b200 as hb
+    front, behind, qbs = 37, 45, 64
+    lens = [150, 70, 200]
+    pr = make_problem(3, lens, lens, hq, hk, d, qbs, kbs, causal, dtype, 0.6, None)
+    total = sum(lens)
+    rest = (pr["cu_q"], pr["cu_k"], pr["mask"], qbs, kbs, causal)
+    _, lse = hb.HBSAttention_with_lse(pr["q"], pr["k"], pr["v"], *rest)
+    lse[:front] = lse[total - behind:] = float("-inf")        # the whole problem without the rows that will be missing
+    hb.set_kernel_family(family)
+    try:
+        want = hb.attention_key_weights(pr["q"], pr["k"], lse, *rest)
+        cut = slice(front, total - behind)
+        cu = pr["cu_q"] - front
+        got = hb.attention_key_weights(pr["q"][cut].clone(), pr["k"][cut].clone(), lse[cut].clone(), cu, cu, *rest[2:])
+        assert hb.last_status()[0] == 0
+        assert torch.equal(got, want[cut])
+        none = torch.zeros_like(pr["mask"])                   # nothing active: zeros for the keys that are there
+        assert not hb.attention_key_weights(pr["q"][cut].clone(), pr["k"][cut].clone(), lse[cut].clone(), cu, cu, none, *rest[3:]).any()
+    finally:
+        hb.set_kernel_family("auto")
