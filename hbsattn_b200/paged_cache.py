@@ -45,7 +45,8 @@ def _same_device(*tensors):
 
 
 def _int32(t):
-    return t if t.dtype == torch.int32 else t.to(torch.int32)
+    """Integers as the kernels want them; what does not fit becomes the nearest that does, and is out of range there too."""
+    return t if t.dtype == torch.int32 else t.to(torch.int64).clamp(-2 ** 31, 2 ** 31 - 1).to(torch.int32)
 
 
 def _check_cache(k_cache, v_cache, block_table, cache_lens):
