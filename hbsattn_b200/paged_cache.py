@@ -49,6 +49,16 @@ def _int32(t):
     return t if t.dtype == torch.int32 else t.to(torch.int64).clamp(-2 ** 31, 2 ** 31 - 1).to(torch.int32)
 
 
+def _is_integer(t):
+    return not t.is_floating_point() and not t.is_complex()
+
+
+def _check_sizes(**sizes):
+    """What goes to the library in 32 bits."""
+    for name, n in sizes.items():
+        assert n < 2 ** 31, f"{name} must fit 31 bits, got {n}"
+
+
 def _check_cache(k_cache, v_cache, block_table, cache_lens):
     """Checks, and ``block_table`` and ``cache_lens`` as the kernels want them."""
     assert k_cache.ndim == 4 and k_cache.shape == v_cache.shape, "k_cache and v_cache must be (num_pages, page_size, nhead_k, headdim)"
@@ -57,7 +67,8 @@ def _check_cache(k_cache, v_cache, block_table, cache_lens):
     assert k_cache.shape[3] <= 256, "headdim above 256 is not supported"
     assert block_table.ndim == 2 and block_table.shape[1] > 0, "block_table must be (batch, max_pages)"
     assert cache_lens.shape == block_table.shape[:1], "cache_lens must have one entry per row of block_table"
-    assert not (block_table.is_floating_point() or cache_lens.is_floating_point()), "block_table and cache_lens must be integer tensors"
+    assert _is_integer(block_table) and _is_integer(cache_lens), "block_table and cache_lens must be integer tensors"
+    _check_sizes(num_pages=k_cache.shape[0], page_size=k_cache.shape[1], nhead_k=k_cache.shape[2], batch=block_table.shape[0])
     assert block_table.shape[1] * k_cache.shape[1] < 2 ** 31 - 4096, "max_pages * page_size must fit 31 bits"
     block_table = _int32(block_table)
     if block_table.stride(1) != 1:
@@ -118,6 +129,7 @@ def append_to_cache(k, v, cu_seqlens, k_cache, v_cache, block_table, cache_lens)
     assert k.ndim == 3 and k.shape == v.shape and k.shape[1:] == k_cache.shape[2:], "k and v must be (total, nhead_k, headdim) like the cache's"
     assert k.dtype == v.dtype == k_cache.dtype, "k and v must have the cache's dtype"
     assert cu_seqlens.ndim == 1 and cu_seqlens.numel() == lens.numel() + 1, "cu_seqlens must be a 1D tensor of length batch + 1"
+    _check_sizes(total=k.shape[0])
     cu = _int32(cu_seqlens).contiguous()
     dev = k.device
     with torch.cuda.device(dev):
@@ -160,11 +172,13 @@ def paged_attention(q, k_cache, v_cache, block_table, cache_lens, softmax_scale=
     assert q.ndim == 3 and q.shape[0] == batch and q.shape[2] == headdim, "q must be (batch, nhead_q, headdim) with the cache's headdim"
     assert q.dtype == k_cache.dtype, "q must have the cache's dtype"
     assert q.shape[1] > 0 and q.shape[1] % nhead_k == 0, "nhead_q must be divisible by nhead_k (for GQA)"
+    _check_sizes(nhead_q=q.shape[1])
     if block_mask is not None:
         assert block_mask.dtype == torch.bool, "block_mask must be a boolean tensor"
         assert k_block_size is not None and k_block_size > 0 and k_block_size % 16 == 0, "k_block_size must be an integer multiple of 16."
         assert block_mask.ndim == 3 and block_mask.shape[:2] == (batch, nhead_k) and block_mask.shape[2] * k_block_size >= capacity, \
             f"block_mask must be ({batch}, {nhead_k}, num_k_block) and cover max_pages * page_size = {capacity} positions"
+        _check_sizes(k_block_size=k_block_size, num_k_block=block_mask.shape[2])
     if key_weights is not None:
         _check_weights(key_weights, batch, nhead_k, capacity)
         _check_writable("paged_attention", key_weights)
@@ -206,6 +220,8 @@ def _key_weights(q, k, lse, cu_q_seqlens, cu_k_seqlens, mask, csr, num_q_block, 
     assert q_block_size % 16 == 0 and k_block_size % 16 == 0 and q_block_size > 0 and k_block_size > 0, \
         "q_block_size and k_block_size must be integer multiples of 16."
     assert lse.dtype == torch.float32 and lse.shape == q.shape[:2], "lse must be float32 [total_q, nhead_q]"
+    _check_sizes(total_q=q.shape[0], total_k=k.shape[0], q_block_size=q_block_size, k_block_size=k_block_size, num_q_block=num_q_block,
+                 num_k_block=num_k_block)
     lse = lse.contiguous()
     lib = _lib.load()
     dev = q.device
@@ -267,9 +283,10 @@ def select_keys(key_weights, cache_lens, budget, n_sink=0, n_recent=0):
     _refuse_gradients("select_keys", key_weights)
     assert key_weights.dtype == torch.float32 and key_weights.ndim == 3 and key_weights.shape[2] > 0, "key_weights must be float32 (batch, nhead_k, positions)"
     assert key_weights.shape[2] < 2 ** 31 - 16384, "the positions must fit 31 bits"
-    assert cache_lens.shape == key_weights.shape[:1] and not cache_lens.is_floating_point(), "cache_lens must be an integer tensor of length batch"
+    assert cache_lens.shape == key_weights.shape[:1] and _is_integer(cache_lens), "cache_lens must be an integer tensor of length batch"
     assert budget > 0 and n_sink >= 0 and n_recent >= 0 and n_sink + n_recent <= budget, \
         "budget must be positive, n_sink and n_recent not negative and together not above budget"
+    _check_sizes(budget=budget, batch=key_weights.shape[0], nhead_k=key_weights.shape[1])
     if key_weights.stride(2) != 1:
         key_weights = key_weights.contiguous()
     lens = _int32(cache_lens).contiguous()
@@ -301,9 +318,10 @@ def compact_cache(k_cache, v_cache, block_table, cache_lens, kept, kept_lens, ke
     block_table, lens = _check_cache(k_cache, v_cache, block_table, cache_lens)
     _check_writable("compact_cache", k_cache, v_cache)
     batch, nhead_k = block_table.shape[0], k_cache.shape[2]
-    assert kept.ndim == 3 and kept.shape[:2] == (batch, nhead_k) and kept.shape[2] > 0 and not kept.is_floating_point(), \
+    assert kept.ndim == 3 and kept.shape[:2] == (batch, nhead_k) and kept.shape[2] > 0 and _is_integer(kept), \
         f"kept must be an integer tensor of shape (batch, nhead_k, budget) = ({batch}, {nhead_k}, ...)"
-    assert kept_lens.shape == lens.shape and not kept_lens.is_floating_point(), "kept_lens must be an integer tensor of length batch"
+    assert kept_lens.shape == lens.shape and _is_integer(kept_lens), "kept_lens must be an integer tensor of length batch"
+    _check_sizes(budget=kept.shape[2])
     if key_weights is not None:
         _check_weights(key_weights, batch, nhead_k, block_table.shape[1] * k_cache.shape[1])
         _check_writable("compact_cache", key_weights)
