@@ -100,13 +100,16 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ App
 // ------------------------------------------------------------------------------------------------------------------
 // Select: radix select of the smallest weight that stays, then one pass that writes positions in order.  The digits are 11 bits of the distance
 // from the smallest weight above zero (or, where all of those stay, from the smallest of the rest): that keeps keys that nobody has looked at
-// out of the counts, where they would meet in one bin, and spreads weights of one size over many.  Where no more weights than threads come down
-// to the next digit (the rule after the first one), each finds its rank among them at once: 20.1 instead of 23.7 us, of 128 rows of 16384 to 32768.
+// out of the counts, where they would meet in one bin, and spreads weights of one size over many.  Where no more than kSelectRank weights come down
+// to the next digit (usual after the first one), each finds its rank among them at once.  Ranking n weights against going on by digits, in us: 128 rows
+// of 24576 17.0 and 19.7 (n = 16), 18.0 and 20.0 (100), 19.1 and 20.1 (150), 27.7 and 20.4 (512), 55.5 and 20.6 (1000); 128 rows of 8192 7.6 and 8.9,
+// 8.4 and 8.9, 9.4 and 9.0, 17.3 and 9.1, 44.2 and 9.1; 16 rows of 1000 5.3 and 6.3, 5.9 and 6.3, 6.9 and 6.4.
 // A cluster of 1 to 4 CTAs per row; counts
 // are exchanged through distributed shared memory.  Every warp has its run of positions, in registers where they fit, as numbers that tell by
 // themselves whether the position competes; where they do not fit, they are read again for every pass.  Bound by the instructions of its
 // passes (20.1 us for 128 rows of 16384 to 32768, 35 us while every pass compared positions): memory is busy for the first one only.
 constexpr int kSelectBins = 2048;
+constexpr int kSelectRank = 128;
 constexpr uint32_t kGoes = 0u, kStays = 0xffffffffu, kZero = 0x80000000u;
 
 // Weights as unsigned numbers in the same order, from 0x007fffff to 0xff800000; both zeros are one (0x80000000), NaN is the next above them all.
@@ -301,7 +304,7 @@ __global__ void __launch_bounds__(THREADS) select_keys_kernel(const __grid_const
       meet();                                            // also: all have read the counts
       prefix = s_prefix;
       need = s_need;
-      if (left > 0 && ctas == 1 && s_here <= THREADS) {  // few have come down to this digit: a thread for each, which counts those above it
+      if (left > 0 && ctas == 1 && s_here <= kSelectRank) {        // few have come down to this digit: a thread for each, which counts those above it
         const uint32_t from = max(prefix, 1u), size = prefix + (1u << left) - from;
         each([&](uint32_t x, int) {
           if (x - from < size) s_hist[atomicAdd(&s_found, 1)] = (int)x;
