@@ -256,8 +256,10 @@ template <int DP>
 cudaError_t launch_heads(const DecodeParams& P, bool dependent, cudaStream_t stream) {
   if (P.chunk_heads == 1) return launch_kernel(decode_f32_kernel<DP, 1>, (unsigned)P.grid, kThreads, 0, dependent, stream, P);
   if (P.chunk_heads == 2) return launch_kernel(decode_f32_kernel<DP, 2>, (unsigned)P.grid, kThreads, 0, dependent, stream, P);
-  if (P.chunk_heads <= 4 || DP == 256) return launch_kernel(decode_f32_kernel<DP, 4>, (unsigned)P.grid, kThreads, 0, dependent, stream, P);
-  return launch_kernel(decode_f32_kernel<DP, DP == 256 ? 4 : 8>, (unsigned)P.grid, kThreads, 0, dependent, stream, P);
+  if constexpr (DP < 256) {                            // (with 256 columns a chunk has up to 4 heads)
+    if (P.chunk_heads > 4) return launch_kernel(decode_f32_kernel<DP, 8>, (unsigned)P.grid, kThreads, 0, dependent, stream, P);
+  }
+  return launch_kernel(decode_f32_kernel<DP, 4>, (unsigned)P.grid, kThreads, 0, dependent, stream, P);
 }
 
 }  // namespace

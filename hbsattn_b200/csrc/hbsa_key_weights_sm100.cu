@@ -37,7 +37,6 @@ template <int D, bool KEYS> struct Shape {
   static constexpr int kTile = KEYS ? 64 : 128;                 // rows of a streamed tile
   static constexpr int kKeys = KEYS ? 128 : 64;                 // stationary keys
   static constexpr int kStages = D == 64 && KEYS ? 3 : 2;
-  static constexpr int kStat = 1;                               // buffers of stationary keys
   // CTAs of an SM, by shared memory (64 columns: registers); four have its tensor memory
   static constexpr int kResident = D == 64 ? (KEYS ? 4 : 3) : D == 128 ? (KEYS ? 3 : 2) : 1;
   // Tiles whose lse is held.  Its Q goes when the product is done, lse is read until the warps free the next tile's buffer of S.  The product
@@ -60,7 +59,7 @@ template <int D, bool KEYS> struct __align__(16) KwControl {
   int limit[Shape<D, KEYS>::kRows][kKwPieces];               // last key that the piece's first token sees
   int4 list[kKwList];                         // {token, q-head, limit, offset in neg_lse / 16}
   float sums[2][kKwEwWarps][kKwCols];
-  unsigned long long item_full[kKwSlots], item_done[kKwSlots], stat_full[Shape<D, KEYS>::kStat], stat_free[Shape<D, KEYS>::kStat];
+  unsigned long long item_full[kKwSlots], item_done[kKwSlots], stat_full, stat_free;
   unsigned long long strm_full[Shape<D, KEYS>::kStages], strm_free[Shape<D, KEYS>::kStages], rows_full[Shape<D, KEYS>::kRows];
   unsigned long long s_full[2], s_free[2], sums_ready[2], drain;
   KwItem slot[kKwSlots];
@@ -69,7 +68,7 @@ template <int D, bool KEYS> struct __align__(16) KwControl {
 };
 
 template <int D, bool KEYS> constexpr size_t kw_smem() {
-  const size_t n = (size_t)Shape<D, KEYS>::kStat * Shape<D, KEYS>::kKeys * D * 2u + (size_t)Shape<D, KEYS>::kStages * Shape<D, KEYS>::kTile * D * 2u + sizeof(KwControl<D, KEYS>);
+  const size_t n = (size_t)Shape<D, KEYS>::kKeys * D * 2u + (size_t)Shape<D, KEYS>::kStages * Shape<D, KEYS>::kTile * D * 2u + sizeof(KwControl<D, KEYS>);
   return n < kKwLeastSmem ? kKwLeastSmem : n;
 }
 static_assert(kw_smem<256, true>() <= 227u * 1024u && kw_smem<256, false>() <= 227u * 1024u, "shared memory of one CTA");
@@ -112,22 +111,20 @@ __global__ void __launch_bounds__(kKwThreads, (Shape<D, KEYS>::kResident))
 key_weights_sm100_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ KeyWeightsParams P) {
   using namespace ptx;
   using S = Shape<D, KEYS>;
-  constexpr int PANELS = D / 64, STAGES = S::kStages, STAT_BUFS = S::kStat, ROWS = S::kRows, TILE = S::kTile;
+  constexpr int PANELS = D / 64, STAGES = S::kStages, ROWS = S::kRows, TILE = S::kTile;
   constexpr uint32_t STAT = (uint32_t)S::kKeys * D * 2u, STRM = (uint32_t)TILE * D * 2u;
   constexpr uint32_t STAT_PANEL = (uint32_t)S::kKeys * 128u, STRM_PANEL = (uint32_t)TILE * 128u;
   const Problem& p = P.p;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   extern __shared__ __align__(1024) uint8_t smem[];
-  const uint32_t sStat = smem_u32(smem), sStrm = sStat + STAT_BUFS * STAT;
-  auto* const ctl = reinterpret_cast<KwControl<D, KEYS>*>(smem + STAT_BUFS * STAT + STAGES * STRM);
+  const uint32_t sStat = smem_u32(smem), sStrm = sStat + STAT;
+  auto* const ctl = reinterpret_cast<KwControl<D, KEYS>*>(smem + STAT + STAGES * STRM);
   volatile int* const abort_flag = &ctl->abort_flag;
   const long long budget = P.wait_budget;
   const uint32_t b_item_full = smem_u32(ctl->item_full), b_item_done = smem_u32(ctl->item_done);
-  const uint32_t b_stat_full = smem_u32(ctl->stat_full), b_stat_free = smem_u32(ctl->stat_free);
+  const uint32_t b_stat_full = smem_u32(&ctl->stat_full), b_stat_free = smem_u32(&ctl->stat_free);
   const uint32_t b_strm_full = smem_u32(ctl->strm_full), b_strm_free = smem_u32(ctl->strm_free), b_rows_full = smem_u32(ctl->rows_full);
   const uint32_t b_s_full = smem_u32(ctl->s_full), b_s_free = smem_u32(ctl->s_free), b_sums = smem_u32(ctl->sums_ready);
-  auto stat_of = [](uint32_t base, int i) { return base + 8u * (uint32_t)(i % STAT_BUFS); };
-  auto stat_par = [](int i) { return (uint32_t)(i / STAT_BUFS) & 1u; };
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(b_item_full + 8 * i, 1);
@@ -136,10 +133,8 @@ key_weights_sm100_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_
       mbar_init(b_s_free + 8 * i, kKwEwWarps);
       mbar_init(b_sums + 8 * i, kKwEwWarps);
     }
-    for (int i = 0; i < STAT_BUFS; ++i) {
-      mbar_init(b_stat_full + 8 * i, 1);
-      mbar_init(b_stat_free + 8 * i, 1);
-    }
+    mbar_init(b_stat_full, 1);
+    mbar_init(b_stat_free, 1);
     for (int i = 0; i < STAGES; ++i) {
       mbar_init(b_strm_full + 8 * i, 1);
       mbar_init(b_strm_free + 8 * i, 1);
@@ -265,13 +260,12 @@ key_weights_sm100_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_
       }
       ++items;
       if (last) break;
-      if (with_tiles >= STAT_BUFS) ok = warp_wait(stat_of(b_stat_free, with_tiles), stat_par(with_tiles - STAT_BUFS), abort_flag, budget);
+      if (with_tiles > 0) ok = warp_wait(b_stat_free, (uint32_t)(with_tiles - 1) & 1u, abort_flag, budget);
       if (!ok) break;
       if (lane == 0) {
-        const uint32_t bar = stat_of(b_stat_full, with_tiles), dst = sStat + (uint32_t)(with_tiles % STAT_BUFS) * STAT;
-        mbar_arrive_expect_tx(bar, (uint32_t)P.n_cols * D * 2u);
+        mbar_arrive_expect_tx(b_stat_full, (uint32_t)P.n_cols * D * 2u);
 #pragma unroll
-        for (int pn = 0; pn < PANELS; ++pn) tma_load_3d(dst + pn * STAT_PANEL, &tm_k, bar, pn * 64, hk, k_begin + k0);
+        for (int pn = 0; pn < PANELS; ++pn) tma_load_3d(sStat + pn * STAT_PANEL, &tm_k, b_stat_full, pn * 64, hk, k_begin + k0);
       }
       ++with_tiles;
 
@@ -355,8 +349,7 @@ key_weights_sm100_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_
       mbar_wait_clock(b_strm_full + 8u * (uint32_t)(c % STAGES), (uint32_t)(c / STAGES) & 1u, budget >> 4);
       mbar_wait_clock(b_rows_full + 8u * (uint32_t)(c % ROWS), (uint32_t)(c / ROWS) & 1u, budget >> 4);
     }
-    for (int back = 1; back <= STAT_BUFS && with_tiles - back >= 0; ++back)
-      mbar_wait_clock(stat_of(b_stat_full, with_tiles - back), stat_par(with_tiles - back), budget >> 4);
+    if (with_tiles > 0) mbar_wait_clock(b_stat_full, (uint32_t)(with_tiles - 1) & 1u, budget >> 4);
   } else if (warp == kKwMma) {
     // =============================== MMA issuer ===============================
     if (lane == 0 && *abort_flag == 0) {
@@ -370,12 +363,12 @@ key_weights_sm100_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_
         const int n = *(volatile int*)&ctl->slot[I & (kKwSlots - 1)].n_tiles;
         mbar_arrive(bar_of(b_item_done, I));
         if (n < 0) break;
-        if (!(ok = mbar_wait_bounded(stat_of(b_stat_full, I), stat_par(I), abort_flag, budget))) break;
+        if (!(ok = mbar_wait_bounded(b_stat_full, (uint32_t)I & 1u, abort_flag, budget))) break;
         for (int t = 0; t < n; ++t, ++T) {
           if (!(ok = mbar_wait_bounded(b_strm_full + 8u * stage, par, abort_flag, budget))) break;
           if (T >= 2 && !(ok = mbar_wait_bounded(bar_of(b_s_free, T), par_of(T - 2), abort_flag, budget))) break;
           tc_fence_after();
-          const uint32_t lq = smem_desc_lo(sStrm + (uint32_t)stage * STRM, 16u), lk = smem_desc_lo(sStat + (uint32_t)(I % STAT_BUFS) * STAT, 16u);
+          const uint32_t lq = smem_desc_lo(sStrm + (uint32_t)stage * STRM, 16u), lk = smem_desc_lo(sStat, 16u);
           const uint32_t la = KEYS ? lk : lq, lb = KEYS ? lq : lk;
           const uint32_t tS = tmem + (uint32_t)((T & 1) * kKwCols);
 #pragma unroll
@@ -387,7 +380,7 @@ key_weights_sm100_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_
           }
           tc_commit(bar_of(b_s_full, T));
           tc_commit(b_strm_free + 8u * stage);
-          if (t == n - 1) tc_commit(stat_of(b_stat_free, I));
+          if (t == n - 1) tc_commit(b_stat_free);
           if (++stage == STAGES) {
             stage = 0;
             par ^= 1u;
