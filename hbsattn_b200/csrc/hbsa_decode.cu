@@ -18,15 +18,6 @@ namespace hbsa {
 
 namespace {
 
-template <typename T> __device__ __forceinline__ float to_f(T x);
-template <> __device__ __forceinline__ float to_f<float>(float x) { return x; }
-template <> __device__ __forceinline__ float to_f<__half>(__half x) { return __half2float(x); }
-template <> __device__ __forceinline__ float to_f<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
-template <typename T> __device__ __forceinline__ T from_f(float x);
-template <> __device__ __forceinline__ float from_f<float>(float x) { return x; }
-template <> __device__ __forceinline__ __half from_f<__half>(float x) { return __float2half_rn(x); }
-template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
-
 // One warp per (sequence, kv-head): its active blocks below the sequence's length, and how many pieces of `unit` positions they
 // have (the last block of the sequence may be short).
 __global__ void __launch_bounds__(256) decode_blocks_kernel(const __grid_constant__ DecodeParams P) {

@@ -91,15 +91,6 @@ template <bool BF16> __device__ __forceinline__ void mma16816(float (&c)[4], con
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// A wait of a whole warp that finds the phase complete, or nearly so.
-__device__ __forceinline__ bool quick_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, long long budget) {
-#pragma unroll 1
-  for (int i = 0; i < 16; ++i)
-    if (__all_sync(0xffffffffu, ptx::mbar_test(bar, parity))) return true;
-  const bool ok = warp_wait(bar, parity, abort_flag, budget);
-  __syncwarp();
-  return ok;
-}
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kThreads, 1)
 decode_sm100_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ DecodeParams P) {

@@ -20,11 +20,6 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kKeys = 64, kRows = 64, kThreads = 256;
 
-template <typename T> __device__ __forceinline__ float to_f(T x);
-template <> __device__ __forceinline__ float to_f<float>(float x) { return x; }
-template <> __device__ __forceinline__ float to_f<__half>(__half x) { return __half2float(x); }
-template <> __device__ __forceinline__ float to_f<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
-
 // The k-blocks by the number of rows that may see them, most first, so that the items that end a launch are short.  One CTA, 256 classes, which are
 // counted in the workspace: shared memory here would keep CTAs of the next kernel from starting beside this one (4 us of 57).
 __device__ __forceinline__ void key_weights_order(const KeyWeightsParams& P) {

@@ -88,12 +88,6 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
-__device__ __forceinline__ bool quick_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, long long budget) {
-  if (__all_sync(0xffffffffu, ptx::mbar_test(bar, parity))) return true;
-  const bool ok = warp_wait(bar, parity, abort_flag, budget);
-  __syncwarp();
-  return ok;
-}
 
 // One step of a sum over the lanes of v[0 .. 2 N): lanes that differ in bit N / 2 exchange halves.  After 32, 16, 8, 4, 2 v[0] and v[1] are
 // columns 2 lane and 2 lane + 1.
