@@ -107,7 +107,8 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ App
 // A cluster of 1 to 4 CTAs per row; counts
 // are exchanged through distributed shared memory.  Every warp has its run of positions, in registers where they fit, as numbers that tell by
 // themselves whether the position competes; where they do not fit, they are read again for every pass.  Bound by the instructions of its
-// passes (20.1 us for 128 rows of 16384 to 32768, 35 us while every pass compared positions): memory is busy for the first one only.
+// passes (20.1 us for 128 rows of 16384 to 32768, 35 us while every pass compared positions): 61 % of the issue slots; no wait stands out, shared
+// atomics take 7 % of the cycles, and memory is busy for the first pass only.
 constexpr int kSelectBins = 2048;
 constexpr int kSelectRank = 128;
 constexpr uint32_t kGoes = 0u, kStays = 0xffffffffu, kZero = 0x80000000u;
@@ -407,7 +408,8 @@ cudaError_t launch_select(const hbsa_select_keys_args& a, int ctas, cudaStream_t
 // Compact: kept positions ascend, so row j comes from row kept[j] >= j, and writing rows [c, d) touches no row that a later chunk still
 // reads.  A CTA takes one slice of the columns of one (sequence, kv-head), of K or of V, chunk by chunk: the rows of the next
 // chunk are read (their positions one chunk before), all threads meet, then the rows of this one are written.
-// Bound by latency where there are few sequences, by memory otherwise (8 x 4096 rows of 8 heads of 128, from 8192 to 32768: 62.4 us, 4.4 TB/s).
+// Bound by the way from chunk to chunk: of 13.6 warps a scheduler 5.3 wait for gathered rows and 2.3 at the meetings (8 x 4096 rows of 8 heads of 128,
+// from 8192 to 32768: 62.4 us, 4.4 TB/s).
 struct CompactParams {
   void* cache[2];
   Rows4 rows[2];
@@ -443,6 +445,7 @@ __device__ __forceinline__ void compact_rows(int n, int row, int rows, Next next
   }
 }
 
+// (64 registers, the 16-byte builds spill 52 bytes)
 template <typename U, int THREADS>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS) compact_kernel(const __grid_constant__ CompactParams P) {
   const int parts = P.slices + (P.weights != nullptr ? 1 : 0);
@@ -616,6 +619,8 @@ int hbsa_select_keys(const hbsa_select_keys_args* a, void* stream) {
   // CTAs of a row: as many (up to 4) as bring them down to 8192 positions each where all of them have an SM, else as few as can hold the row.
   // 16 rows of 32768 by 1, 2 and 4 CTAs: 19.7, 22.5 and 15.8 us (by 8: 47, clusters of eight full SMs do not find their places at once);
   // 16 of 9000 by 1 and 2: 15.2 and 13.1 us; 8 of 8192 by 1 and 2: 7.4 and 13.3 us.
+  // The lengths are on the device, so this goes by the width of the weights.  Short rows in a wide tensor pay for it: 128 rows of 4000 take 7.7 us
+  // in 8192 columns, 13.7 in 32768, 39 in 65536 and 91 in 131072 and more; cut the tensor to the longest sequence where that is known.
   const long long rows = (long long)a->batch * a->nhead_k;
   auto split = [&](int most) {
     int n = 1;

@@ -6,8 +6,10 @@
 // another warp before the row of heads ends.  The products of a slab are sums over the lanes: lanes exchange halves of what they
 // have and add, log2(32) times, after which every (key, head) is in a lane of its own: one shuffle a sum, and one exponential a lane.
 // Its probability goes back to all lanes by shuffles for O += P V, whose columns stay where V's are.
-// Up to 8 heads (4 with 256 columns) share the read of K and V; groups of more take several chunks.
-// With 16 warps an SM, each with up to 8 KB on its way, the read of K and V bounds it for small groups, the instructions for larger ones:
+// Up to 8 heads (4 with 256 columns) share the read of K and V; groups of more take several chunks, each of which reads K and V again (8 x 8192 keys, 4
+// kv-heads of 256: 87, 106 and 191 us with groups of 1, 4 and 8).
+// With 16 warps an SM, each with up to 8 KB on its way, the read of K and V bounds it for small groups, for larger ones
+// the instructions (62 % of the issue slots and 36 % of the FMA pipe with groups of 8, where a slab's read also waits for the products of the one before):
 // 8 x 8192..16384 keys, 8 heads of 128, take 123, 154 and 230 us with groups of 1, 4 and 8 (6.4, 5.1 and 3.4 TB/s).  The kernel with tiles
 // in shared memory meets five times a tile: 490 us with groups of 4.
 #include "hbsa_decode.cuh"
@@ -30,8 +32,9 @@ template <int DP, int HEADS>
 __global__ void __launch_bounds__(kThreads, 2) decode_f32_kernel(const __grid_constant__ DecodeParams P) {
   constexpr int LPK = DP >= 128 ? 32 : DP / 4;         // lanes of a key
   constexpr int UNITS = DP / (4 * LPK);                // 16-byte units of a lane
-  // keys of a slab, and of a lane: as many as registers hold (8 heads of 128 with slabs of 8 and 4: 351 and 230 us for 8 x 8192..16384 keys, 4 heads
-  // of 256 with slabs of 4 and 2: 159 and 134 us for half of them)
+  // keys of a slab, and of a lane, by measurement (8 heads of 128 with slabs of 8 and 4: 351 and 230 us for 8 x 8192..16384 keys, 4 heads of 256
+  // with slabs of 4 and 2: 159 and 134 us for half of them).  Registers hold that nearly: at 128 a thread six of the eleven instances spill, 8 heads of
+  // 64 and 128 244 and 188 bytes, the others up to 52.
   constexpr int SLAB = DP == 256 ? (HEADS == 4 ? 2 : 4) : DP == 128 && HEADS == 8 ? 4 : 8, KPL = SLAB / (32 / LPK);
   constexpr int N = KPL * HEADS;                       // sums of a group of LPK lanes: sum v = key * HEADS + head ends in lane v / R * REP
   constexpr int R = N > LPK ? N / LPK : 1, REP = N < LPK ? LPK / N : 1;    // sums of a lane, lanes of a sum

@@ -13,8 +13,10 @@
 //               all of its columns where headdim is a multiple of 64 (x, slot, panel), one per panel of 64 columns otherwise.
 //   warps 0-7   warp w takes a slab of 16 or 32 keys of a stage, the (w mod 4)-th: S = Q K^T (16 heads), running maximum and sum, O += P V.
 //               With up to 16 heads warps 0-3 take the even stages and 4-7 the odd ones, with up to 32 both take every stage, 16
-//               heads each.  256 columns of O do not fit a warp's registers: there both take every stage, up to 16 heads and half
-//               of O's columns each (the scores are made twice), and Q is read from shared memory for every product.
+//               heads each (groups of more take several chunks, each of which reads K and V again: 8 x 16384 keys, 4 kv-heads of 128: 86 us with groups
+//               of 32, 133 with 64).  256 columns of O do not fit a warp's registers: there both take every stage, up to 16 heads (chunks of 16:
+//               groups of 16 and 32 of 256 columns 101 and 175 us) and half of O's columns each (the scores are made twice), and Q is read from
+//               shared memory for every product.
 // At the end of a row the warps' parts are put together through shared memory, up to 128 columns at a time.
 // P enters P V in the type of V, as in the prompt's kernels: at most 2^-8 (bf16) or 2^-11 (fp16) of a term, what the rounding of the output costs too (bf16
 // over 16384..32768 keys: 1.8e-3 of the output against 64 bits, 1.6e-3 with P in fp32).  In fp16 that holds for normal numbers only, so P is formed
