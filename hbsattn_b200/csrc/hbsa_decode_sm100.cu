@@ -18,12 +18,16 @@
 //               groups of 16 and 32 of 256 columns 101 and 175 us) and half of O's columns each (the scores are made twice), and Q is read from
 //               shared memory for every product.
 // At the end of a row the warps' parts are put together through shared memory, up to 128 columns at a time.
-// P enters P V in the type of V, as in the prompt's kernels: at most 2^-8 (bf16) or 2^-11 (fp16) of a term, what the rounding of the output costs too (bf16
-// over 16384..32768 keys: 1.8e-3 of the output against 64 bits, 1.6e-3 with P in fp32).  In fp16 that holds for normal numbers only, so P is formed
-// against the maximum less 14 there: the largest is 2^14 (of 2^16 that fp16 has), and rounding is by 2^-11 of a term down to 2^-28 of the largest, by at most
-// 2^-39 of the largest below.  Against the maximum itself everything below 2^-25 was lost (equal keys 19 nats below sinks that every
-// warp meets: all of their share; now within 2^-10 of it, in the same time).  The factor is in O, the sums and the maxima that are handed on, and
-// leaves with the division.  Scores, statistics and sums are fp32.
+// P enters P V in the type of V.  With up to 8 heads a chunk it does so in two terms, P rounded and what that leaves (as in the package's backward): rows
+// 8 to 15 of the products' left operands, which would be idle, hold the second term, and the two halves of O come together at the end of the row.  That
+// costs nothing (16 x 16384..32768 keys, 8 heads of 64, groups of 8: 128.1 us, with one term 128.9; 8 x 16384..65536 at 30 % 100.7 and 100.5; fp16 with
+// weights 30.8 and 32.3, as no exponentials are made for the idle rows) and takes P's rounding out of the result: 1.65e-3 (bf16) and 2.1e-4 (fp16) of
+// the output against 64 bits, what the output's own rounding makes; 2.1e-3 to 2.2e-3 and 2.7e-4 with one term (8 x 4096..16384 keys).  More heads use
+// all rows and have one term, at most 2^-8 or 2^-11 of every p, like the prompts' kernels: a second product would double the tensor work.
+// In fp16 such bounds hold for normal numbers only, so P is formed against the maximum less 14 there: the largest is 2^14 (of 2^16 that
+// fp16 has), and rounding is by 2^-11 of a term down to 2^-28 of the largest, by at most 2^-39 of the largest below.  Against the maximum itself
+// everything below 2^-25 was lost (equal keys 19 nats below sinks that every warp meets: all of their share; now within 2^-10 of it, in the same time).
+// The factor is in O, the sums and the maxima that are handed on, and leaves with the division.  Scores, statistics and sums are fp32.
 // Measured: 16 x 16384..32768 keys, 8 heads of 64, groups of 8: 125 us, of which 102 are the stream (745 MB, 7.3 TB/s), 6 the way to the first tile, 6
 // the join; 8 x 16384..65536 keys, 30 % of the blocks, 8 heads of 128: 98 us (527 MB).  A call without work to speak of: 10.5 us.
 // Positions behind the length share the last tile with others and may hold anything: their scores are set to -inf, and their
@@ -93,7 +97,8 @@ template <bool BF16> __device__ __forceinline__ void mma16816(float (&c)[4], con
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-template <int D, bool BF16>
+// PAIRED: up to 8 heads a chunk, rows 8 .. 15 hold what P of rows 0 .. 7 loses in 16 bits.
+template <int D, bool BF16, bool PAIRED>
 __global__ void __launch_bounds__(kThreads, 1)
 decode_sm100_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ DecodeParams P) {
   using namespace ptx;
@@ -293,7 +298,7 @@ decode_sm100_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
       float *score0 = nullptr, *score1 = nullptr;
       if (P.weights != nullptr) {
         if (head_base + g < heads) score0 = P.sp.scores + ((long long)r.b * P.nhead_q + head0 + head_base + g) * P.capacity;
-        if (head_base + g + 8 < heads) score1 = P.sp.scores + ((long long)r.b * P.nhead_q + head0 + head_base + g + 8) * P.capacity;
+        if (!PAIRED && head_base + g + 8 < heads) score1 = P.sp.scores + ((long long)r.b * P.nhead_q + head0 + head_base + g + 8) * P.capacity;
       }
       // a stage holds the same number of pieces whatever the row's first tile is, so the last one of a row may be half empty, and
       // of every 32 pieces that are looked up together the last stage is full
@@ -358,7 +363,7 @@ decode_sm100_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
 #pragma unroll
             for (int j = 0; j < 2 * UNITS; ++j) {
               x0 = fmaxf(x0, fmaxf(s[j][0], s[j][1]));
-              x1 = fmaxf(x1, fmaxf(s[j][2], s[j][3]));
+              if (!PAIRED) x1 = fmaxf(x1, fmaxf(s[j][2], s[j][3]));
             }
             if (__any_sync(0xffffffffu, x0 > m0 || x1 > m1)) {       // some row's maximum grows: the quads agree on it, O and the sums follow
               x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 1));
@@ -366,7 +371,8 @@ decode_sm100_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
               x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 2));
               x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 2));
               // (the references' difference is not the maxima's: subtracting 14 may round)
-              const float a0 = x0 == -INFINITY ? 1.f : ex2_approx(reference(m0) - reference(x0)), a1 = x1 == -INFINITY ? 1.f : ex2_approx(reference(m1) - reference(x1));
+              const float a0 = x0 == -INFINITY ? 1.f : ex2_approx(reference(m0) - reference(x0));
+              const float a1 = PAIRED ? a0 : x1 == -INFINITY ? 1.f : ex2_approx(reference(m1) - reference(x1));
               l0 *= a0;
               l1 *= a1;
 #pragma unroll
@@ -383,11 +389,16 @@ decode_sm100_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
             uint32_t p[UNITS][4];
 #pragma unroll
             for (int j = 0; j < 2 * UNITS; ++j) {
-              const float p0 = ex2_approx(s[j][0] - r0), p1 = ex2_approx(s[j][1] - r0), p2 = ex2_approx(s[j][2] - r1), p3 = ex2_approx(s[j][3] - r1);
+              const float p0 = ex2_approx(s[j][0] - r0), p1 = ex2_approx(s[j][1] - r0);
               l0 += p0 + p1;
-              l1 += p2 + p3;
-              p[j >> 1][2 * (j & 1)] = pack2<BF16>(p0, p1);
-              p[j >> 1][2 * (j & 1) + 1] = pack2<BF16>(p2, p3);
+              if (PAIRED) {
+                split2<BF16>(p0, p1, p[j >> 1][2 * (j & 1)], p[j >> 1][2 * (j & 1) + 1]);
+              } else {
+                const float p2 = ex2_approx(s[j][2] - r1), p3 = ex2_approx(s[j][3] - r1);
+                l1 += p2 + p3;
+                p[j >> 1][2 * (j & 1)] = pack2<BF16>(p0, p1);
+                p[j >> 1][2 * (j & 1) + 1] = pack2<BF16>(p2, p3);
+              }
             }
             if (least < 16) {                        // rows of V that take no part: zeros
 #pragma unroll
@@ -437,14 +448,23 @@ decode_sm100_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
       // Up to 8 heads: rows 0-7 of each warp, 128 columns (or all) at a time; else 16 rows, 64 columns.  Nobody waits but for the writers: 1.3 us a
       // row, 4.6 with one meeting before and one after every exchange of 64 columns.
       if (HALVES) part_read();                       // Q
-      const bool few = heads <= 8;
+      if (PAIRED) {
+#pragma unroll
+        for (int i = 0; i < COLUMNS / 8; ++i)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {              // (an infinite value times a rest that is zero or negative: the first term alone is right)
+            const float both = o[i][e] + o[i][2 + e];
+            o[i][e] = both == both ? both : o[i][e];
+          }
+      }
+      const bool few = PAIRED || heads <= 8;
       const int width = few && COLUMNS >= 128 ? 128 : 64, rows = few ? 8 : 16;
       const long long part_slot = 2ll * blockIdx.x + max(r.slot, 0);
       for (int c0 = 0; c0 < COLUMNS; c0 += width) {
         if (!(ok = part_writable())) break;
         if (t4 == 0) {
           *reinterpret_cast<float2*>(ctl->ml[warp][g]) = make_float2(reference(m0), l0);
-          *reinterpret_cast<float2*>(ctl->ml[warp][g + 8]) = make_float2(reference(m1), l1);
+          if (!PAIRED) *reinterpret_cast<float2*>(ctl->ml[warp][g + 8]) = make_float2(reference(m1), l1);
         }
 #pragma unroll
         for (int i = 0; i < COLUMNS / 8; ++i) {
@@ -527,12 +547,17 @@ bool encode_cache_map(EncodeTiledFn fn, CUtensorMap* map, bool bf16, const void*
             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, promotion, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int D, bool BF16>
+template <int D, bool BF16, bool PAIRED>
 cudaError_t launch_one(const CUtensorMap& tk, const CUtensorMap& tv, const DecodeParams& P, bool dependent, cudaStream_t stream) {
   static SmemOptIn opt_in;
-  cudaError_t e = opt_in.once(reinterpret_cast<const void*>(decode_sm100_kernel<D, BF16>), (int)decode_smem<D>());
+  cudaError_t e = opt_in.once(reinterpret_cast<const void*>(decode_sm100_kernel<D, BF16, PAIRED>), (int)decode_smem<D>());
   if (e != cudaSuccess) return e;
-  return launch_kernel(decode_sm100_kernel<D, BF16>, (unsigned)P.grid, kThreads, decode_smem<D>(), dependent, stream, tk, tv, P);
+  return launch_kernel(decode_sm100_kernel<D, BF16, PAIRED>, (unsigned)P.grid, kThreads, decode_smem<D>(), dependent, stream, tk, tv, P);
+}
+
+template <int D, bool BF16>
+cudaError_t launch_heads(const CUtensorMap& tk, const CUtensorMap& tv, const DecodeParams& P, bool dependent, cudaStream_t stream) {
+  return P.chunk_heads <= 8 ? launch_one<D, BF16, true>(tk, tv, P, dependent, stream) : launch_one<D, BF16, false>(tk, tv, P, dependent, stream);
 }
 
 }  // namespace
@@ -563,9 +588,9 @@ int launch_decode_sm100(const DecodeParams& P, const hbsa_paged_attention_args& 
     return HBSA_ERR_UNSUPPORTED;
   }
   cudaError_t e;
-  if (P.d_pad == 64) e = bf16 ? launch_one<64, true>(tk, tv, P, dependent, stream) : launch_one<64, false>(tk, tv, P, dependent, stream);
-  else if (P.d_pad == 128) e = bf16 ? launch_one<128, true>(tk, tv, P, dependent, stream) : launch_one<128, false>(tk, tv, P, dependent, stream);
-  else e = bf16 ? launch_one<256, true>(tk, tv, P, dependent, stream) : launch_one<256, false>(tk, tv, P, dependent, stream);
+  if (P.d_pad == 64) e = bf16 ? launch_heads<64, true>(tk, tv, P, dependent, stream) : launch_heads<64, false>(tk, tv, P, dependent, stream);
+  else if (P.d_pad == 128) e = bf16 ? launch_heads<128, true>(tk, tv, P, dependent, stream) : launch_heads<128, false>(tk, tv, P, dependent, stream);
+  else e = bf16 ? launch_heads<256, true>(tk, tv, P, dependent, stream) : launch_heads<256, false>(tk, tv, P, dependent, stream);
   if (e != cudaSuccess) { *err_text = cudaGetErrorString(e); return (int)e; }
   return 0;
 }

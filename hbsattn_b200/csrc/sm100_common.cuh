@@ -16,6 +16,26 @@ template <bool BF16> __device__ __forceinline__ uint32_t pack2(float lo, float h
   return r;
 }
 
+template <bool BF16> __device__ __forceinline__ void unpack16(uint32_t w, float& a, float& b) {
+  if (BF16) {
+    a = __uint_as_float(w << 16);
+    b = __uint_as_float(w & 0xffff0000u);
+  } else {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    a = f.x;
+    b = f.y;
+  }
+}
+// x0, x1 = hi + lo, two 16-bit terms each
+template <bool BF16> __device__ __forceinline__ void split2(float x0, float x1, uint32_t& hi, uint32_t& lo) {
+  hi = pack2<BF16>(x0, x1);
+  float h0, h1;
+  unpack16<BF16>(hi, h0, h1);
+  float l0, l1;
+  ptx::unpack_f32x2(ptx::fma_f32x2(ptx::pack_f32x2(h0, h1), ptx::pack_f32x2(-1.f, -1.f), ptx::pack_f32x2(x0, x1)), l0, l1);
+  lo = pack2<BF16>(l0, l1);
+}
+
 // One lane polls the mbarrier, the rest of the warp sleeps at the shuffle instead of spinning.
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, long long budget) {
   int ok = 1;
